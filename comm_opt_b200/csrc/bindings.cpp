@@ -335,6 +335,7 @@ std::vector<int64_t> py_fused_gemm_plan(int64_t M, int64_t N, int64_t K, int64_t
 }  // namespace
 
 void register_ops(pybind11::module& m);  // ops_bindings.cpp
+void register_serve(pybind11::module& m);  // serve_bindings.cpp
 void register_ipc(pybind11::module& m);  // ipc_bindings.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -371,5 +372,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         [](int64_t bn, int64_t splits) { return (int64_t)cob::ar_norm_gemm_resident_clusters((int)bn, (int)splits); });
   m.def("fused_ar_config", &py_fused_ar_config);
   register_ops(m);
+  register_serve(m);
   register_ipc(m);
 }

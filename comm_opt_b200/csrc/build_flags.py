@@ -11,5 +11,6 @@ if os.environ.get("COB_CHECKED"):  # range-checked heap accesses in the collecti
     NVCC.append("-DCOB_CHECKED")
 CXX = ["-O3", "-std=c++17"]
 
-CUDA_SOURCES = ["fused_ar.cu", "fused_gemm.cu", "decode_ops.cu", "attention.cu", "gemm_sm100.cu", "probes.cu"]
-SOURCES = ["bindings.cpp", "ops_bindings.cpp", "ipc_bindings.cpp", "tma_host.cpp"] + CUDA_SOURCES
+CUDA_SOURCES = ["fused_ar.cu", "fused_gemm.cu", "decode_ops.cu", "attention.cu", "gemm_sm100.cu", "probes.cu",
+                "rotary.cu", "logits.cu", "tree_attention.cu"]
+SOURCES = ["bindings.cpp", "ops_bindings.cpp", "serve_bindings.cpp", "ipc_bindings.cpp", "tma_host.cpp"] + CUDA_SOURCES

@@ -426,7 +426,9 @@ Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_
   p.num_blocks = (int)k_cache.size(0);
   p.scale = (float)scale;
   p.dtype = dtype;
-  ok(cob::tree_attention(p, cur()), "tree_attention");
+  // partials of rows cut between CTAs: memory of this call (or of the graph that captures it)
+  Tensor scratch = torch::empty({(int64_t)cob::tree_attention_scratch_bytes(p)}, q.options().dtype(torch::kByte).requires_grad(false));
+  ok(cob::tree_attention(p, scratch.data_ptr(), cur()), "tree_attention");
   return y;
 }
 

@@ -93,6 +93,8 @@ struct TreeAttnParams {
   float scale = 1.f;
   int dtype = 0;
 };
-cudaError_t tree_attention(const TreeAttnParams& p, cudaStream_t s);
+// `scratch`: tree_attention_scratch_bytes(p) bytes, 16-byte aligned, of this call alone; any content.
+size_t tree_attention_scratch_bytes(const TreeAttnParams& p);
+cudaError_t tree_attention(const TreeAttnParams& p, void* scratch, cudaStream_t s);
 
 }  // namespace cob

@@ -34,7 +34,8 @@ namespace {
 using namespace sm100;
 
 constexpr int kPage = 16, kTile = 128, kTilePages = kTile / kPage;
-constexpr int kMaxBatch = 256;  // sequences of one launch (their tile counts are scanned in shared memory)
+constexpr int kMaxBatch = 128;  // sequences of one launch (their lengths and tile counts live in shared memory)
+constexpr int kPieceCost = 2;   // of starting and ending a piece of a (sequence, KV head), in tiles
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint64_t kTimeout = 1000000000ull;  // of every wait, ns
 
@@ -94,11 +95,38 @@ __device__ __forceinline__ uint64_t desc_n_sw128(uint32_t addr, uint32_t lbo) {
   return d;
 }
 constexpr uint32_t kBNMajor = 1u << 16;  // instruction descriptor: B is N-major
+constexpr uint32_t kNegateA = 1u << 13;  // instruction descriptor: A enters with its sign changed
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 16 bytes global -> shared without registers, zeros where `real` is false (nothing is read then)
+__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -122,6 +150,39 @@ constexpr uint32_t kExpMask = 0x7C00u;  // exponent bits of __half: all set in i
 template <>
 constexpr uint32_t kExpMask<__nv_bfloat16> = 0x7F80u;
 
+// zeroes the non-finite halves of a vector; non-zero if there were any
+template <typename T>
+__device__ __forceinline__ uint32_t drop_odd(uint4& v) {
+  uint32_t odd = 0;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    if ((w[x] & kExpMask<T>) == kExpMask<T>) w[x] &= 0xFFFF0000u, odd = 1;
+    if (((w[x] >> 16) & kExpMask<T>) == kExpMask<T>) w[x] &= 0x0000FFFFu, odd = 1;
+  }
+  return odd;
+}
+
+// 4 x 4 vectors across the lanes of a quad, transposed: v[j] becomes lane j's v[this lane's place in the quad]
+__device__ __forceinline__ void quad_transpose(uint4 (&v)[4], int lane) {
+  auto swap = [&](uint4& a, uint4& b, int bit) {  // lanes with the bit clear give b and get a's mate, the others the reverse
+    const bool up = lane & bit;
+    uint4 s = up ? a : b;
+    s.x = __shfl_xor_sync(0xffffffffu, s.x, bit);
+    s.y = __shfl_xor_sync(0xffffffffu, s.y, bit);
+    s.z = __shfl_xor_sync(0xffffffffu, s.z, bit);
+    s.w = __shfl_xor_sync(0xffffffffu, s.w, bit);
+    if (up)
+      a = s;
+    else
+      b = s;
+  };
+  swap(v[0], v[1], 1);
+  swap(v[2], v[3], 1);
+  swap(v[0], v[2], 2);
+  swap(v[1], v[3], 2);
+}
+
 // Bounded wait of a whole warp, one verdict for all lanes (and reconverged: the TMEM accesses that follow need it).
 // Every waiter of a barrier sees every phase of it in turn, so the parity is never ambiguous.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* fail) {
@@ -141,7 +202,7 @@ struct Geo {
   static constexpr int KS = 3, VS = NT == 2 ? 2 : 3;      // ring stages (227 KB per CTA at D = 128)
   static constexpr int WARPS = 4 * NT + 3;
   static constexpr int THREADS = WARPS * 32;
-  static constexpr int SMEM = 1024 + NT * TILE_BYTES + (KS + VS) * TILE_BYTES + 256 + (kMaxBatch + 1) * 4;
+  static constexpr int SMEM = 1024 + NT * TILE_BYTES + (KS + VS) * TILE_BYTES + 256 + (3 * kMaxBatch + 1) * 4;
   static constexpr uint32_t S0 = 0, S1 = 128, O0 = 256;   // TMEM columns
 };
 
@@ -149,53 +210,92 @@ struct alignas(64) TreeArgs {
   CUtensorMap tk, tv;  // caches as [num_blocks * nkv * 16, D], box 16 x 64, 128-byte swizzle
   TreeAttnParams p;
   int group;           // G = nq / nkv
+  uint32_t group_inv;  // ceil(2^32 / G): row / G = high word of row * group_inv (rows * G < 2^32); 0 for G = 1
   int rb;              // row blocks of a (sequence, KV head)
-  int shares;          // equal shares of the flattened (sequence, KV head, tile) space
-  int* cum;            // [batch + 1] scanned tile counts, for the joining kernel
-  float* part_o;       // [shares * rb][2][ROWS][D]
+  int shares;          // equal shares of the flattened (sequence, KV head, piece cost + tile) space
+  float* part_o;       // [shares * rb][2][D / 4][ROWS][4]
   float* part_ml;      // [shares * rb][2][ROWS][2]: maximum (times c) and sum
 };
 
 struct SeqLen {
   int ctx, tl, len;  // cached tokens, drafted tokens, slots in all
 };
-__device__ __forceinline__ SeqLen seq_len(const TreeAttnParams& p, int b) {
+__device__ __forceinline__ SeqLen seq_len(const TreeAttnParams& p, int ctx, int tl) {
   SeqLen s;
   const int cap = p.max_blocks * kPage;
-  s.tl = p.tree_lens ? min(max(p.tree_lens[b], 0), p.tree) : p.tree;
-  s.ctx = min(max(p.ctx_lens[b], 0), cap);
+  s.tl = min(max(tl, 0), p.tree);
+  s.ctx = min(max(ctx, 0), cap);
   s.len = min(s.ctx + s.tl, cap);
   return s;
 }
+__device__ __forceinline__ int token_of(int row, uint32_t inv) { return inv ? (int)__umulhi((uint32_t)row, inv) : row; }
 __device__ __forceinline__ int tiles_of(const SeqLen& s) { return s.tl > 0 ? (s.len + kTile - 1) / kTile : 0; }
+
+// The batch's lengths, and the positions of its work: (sequence b, KV head h) covers the positions
+// [cum[b] + h * (kPieceCost + tiles), ...), kPieceCost of them for starting it and one for every tile.
+struct Lens {
+  int *ctx, *tl, *cum;  // [kMaxBatch], [kMaxBatch], [kMaxBatch + 1]
+  __device__ __forceinline__ explicit Lens(int* mem) : ctx(mem), tl(mem + kMaxBatch), cum(mem + 2 * kMaxBatch) {}
+  __device__ __forceinline__ SeqLen at(const TreeAttnParams& p, int b) const { return seq_len(p, ctx[b], tl[b]); }
+  // by the whole block; ends with a barrier
+  __device__ __forceinline__ void fill(const TreeAttnParams& p) {
+    for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
+      ctx[b] = p.ctx_lens[b];
+      tl[b] = p.tree_lens ? p.tree_lens[b] : p.tree;
+      const int t = tiles_of(at(p, b));
+      cum[b + 1] = t ? (t + kPieceCost) * p.nkv : 0;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const int lane = threadIdx.x;
+      int carry = 0;
+      if (lane == 0) cum[0] = 0;
+      for (int i0 = 0; i0 < p.batch; i0 += 32) {
+        int v = i0 + lane < p.batch ? cum[i0 + lane + 1] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += u;
+        }
+        v += carry;
+        if (i0 + lane < p.batch) cum[i0 + lane + 1] = v;
+        carry = __shfl_sync(0xffffffffu, v, 31);
+      }
+    }
+    __syncthreads();
+  }
+};
 
 // One contiguous piece of a share: tiles [t0, t1) of (b, kvh), of nt in all.
 struct Segment {
   int b, kvh, t0, t1, nt;
-  bool first;  // starts where the share starts (partial slot 0, else 1)
+  bool first;  // of the (sequence, KV head) that holds the share's first position (partial slot 0, else 1)
 };
 struct Walk {
   const int* cum;
   int batch, nkv, g, beg, end;
   __device__ __forceinline__ bool next(Segment& s) {
-    if (g >= end) return false;
-    int lo = 0, hi = batch - 1;  // last b with cum[b] <= g
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (cum[mid] <= g)
-        lo = mid;
-      else
-        hi = mid - 1;
+    while (g < end) {
+      int lo = 0, hi = batch - 1;  // last b with cum[b] <= g
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cum[mid] <= g)
+          lo = mid;
+        else
+          hi = mid - 1;
+      }
+      const int cost = (cum[lo + 1] - cum[lo]) / nkv, rem = g - cum[lo];
+      s.b = lo;
+      s.nt = cost - kPieceCost;
+      s.kvh = rem / cost;
+      const int at = g - (rem - s.kvh * cost);  // position of the (sequence, KV head)
+      s.t0 = max(0, g - at - kPieceCost);
+      s.t1 = min(s.nt, end - at - kPieceCost);
+      s.first = g == beg;
+      g = min(end, at + cost);
+      if (s.t0 < s.t1) return true;  // (a share may end inside the starting cost)
     }
-    s.b = lo;
-    s.nt = (cum[lo + 1] - cum[lo]) / nkv;
-    const int rem = g - cum[lo];
-    s.kvh = rem / s.nt;
-    s.t0 = rem - s.kvh * s.nt;
-    s.t1 = min(s.nt, s.t0 + (end - g));
-    s.first = g == beg;
-    g += s.t1 - s.t0;
-    return true;
+    return false;
   }
 };
 __device__ __forceinline__ int share_beg(int c, int total, int shares) { return (int)((long long)c * total / shares); }
@@ -218,14 +318,15 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
   uint64_t* v_full = k_empty + C::KS;
   uint64_t* v_empty = v_full + C::VS;
   uint64_t* s_full = v_empty + C::VS;  // [2] scores of a buffer are in TMEM
-  uint64_t* p_ready = s_full + 2;      // [2] weights of a buffer are in TMEM
+  uint64_t* p_low = s_full + 2;        // [2] weights of a buffer's first half are in TMEM
+  uint64_t* p_ready = p_low + 2;       // [2] and those of the second
   uint64_t* o_done = p_ready + 2;      // [NT] one more P V of a row tile has completed
   uint64_t* q_ready = o_done + 2;      // [NT] query tile staged
   uint64_t* drain = q_ready + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* s_fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_odd = reinterpret_cast<int*>(tmem_slot + 2);  // a drafted v of this segment is not finite
-  int* cum = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(k_full) + 256);
+  Lens lens(reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(k_full) + 256));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int WK = 4 * NT, WV = WK + 1, WM = WK + 2;
@@ -234,6 +335,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     for (int i = 0; i < C::VS; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
+      mbar_init(&p_low[i], 4);
       mbar_init(&p_ready[i], 4);
       mbar_init(&o_done[i], 1);
       mbar_init(&q_ready[i], 4);
@@ -247,34 +349,15 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
   }
   if (warp == WM) tmem_alloc(tmem_slot, 512);
   pdl_wait_then_trigger();
-  for (int i = threadIdx.x; i < p.batch; i += C::THREADS) cum[i + 1] = tiles_of(seq_len(p, i)) * p.nkv;
   tc_fence_before();
-  __syncthreads();
-  if (warp == 0) {
-    int carry = 0;
-    if (lane == 0) cum[0] = 0;
-    for (int i0 = 0; i0 < p.batch; i0 += 32) {
-      int v = i0 + lane < p.batch ? cum[i0 + lane + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-      }
-      v += carry;
-      if (i0 + lane < p.batch) cum[i0 + lane + 1] = v;
-      carry = __shfl_sync(0xffffffffu, v, 31);
-    }
-  }
-  __syncthreads();
+  lens.fill(p);
   tc_fence_after();
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= p.batch; i += C::THREADS) args.cum[i] = cum[i];
   const uint32_t tmem = *tmem_slot;
-  const int total = cum[p.batch];
+  const int total = lens.cum[p.batch];
   const int share = (int)blockIdx.x / args.rb, rblk = (int)blockIdx.x - share * args.rb;
   const int shares = min(args.shares, total);  // no share is empty, the CTAs past them are idle
   const int beg = share < shares ? share_beg(share, total, shares) : 0, end = share < shares ? share_beg(share + 1, total, shares) : 0;
-  Walk walk{cum, p.batch, p.nkv, beg, beg, end};
+  Walk walk{lens.cum, p.batch, p.nkv, beg, beg, end};
   Segment sg;
 
   if (warp == WK || warp == WV) {
@@ -288,7 +371,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     int st = 0, ph = 0, issued = 0;
     bool okay = true;
     while (okay && walk.next(sg)) {
-      const SeqLen sl = seq_len(p, sg.b);
+      const SeqLen sl = lens.at(p, sg.b);
       const int pages = (sl.len + kPage - 1) / kPage;
       const int* bt = p.block_tables + (size_t)sg.b * p.max_blocks;
       auto entry = [&](int t) {
@@ -318,7 +401,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
   } else if (warp == WM) {
     // ------------------------------------------------ MMAs: S(n) = Q K^T into buffer n & 1, O += P(n) V
     if (lane == 0) {
-      constexpr uint32_t id_qk = idesc_f16(128, kTile, BF16), id_pv = idesc_f16(128, D, BF16) | kBNMajor;
+      const uint32_t id_qk = idesc_f16(128, kTile, BF16) | (p.scale < 0.f ? kNegateA : 0u);
+      constexpr uint32_t id_pv = idesc_f16(128, D, BF16) | kBNMajor;
       int n0 = 0, i0 = 0, seg = 0;  // row-tile steps, KV tiles and segments before this segment
       bool okay = true;
       while (okay && walk.next(sg)) {
@@ -344,17 +428,21 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
         okay = qk(0) && (steps < 2 || qk(1));
         for (int m = 0; m < steps && okay; ++m) {
           const int n = n0 + m, i = i0 + m / NT, st = i % C::VS, tile = m % NT;
-          if (!mbar_wait(&p_ready[n & 1], (n >> 1) & 1, kTimeout) || !mbar_wait(&v_full[st], (i / C::VS) & 1, kTimeout) ||
-              *s_fail) {
-            okay = false;
-            break;
-          }
-          tc_fence_after();
           const uint32_t a = tmem + ((n & 1) ? C::S1 : C::S0), b = smem_addr(sV + st * C::TILE_BYTES);
           const uint32_t d = tmem + C::O0 + tile * D;
+          okay = mbar_wait(&p_low[n & 1], (n >> 1) & 1, kTimeout) && mbar_wait(&v_full[st], (i / C::VS) & 1, kTimeout) &&
+                 *s_fail == 0;
+          if (!okay) break;
+          tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk)
+          for (int kk = 0; kk < kTile / 32; ++kk)
             mma_ts(d, a + kk * 8, desc_n_sw128(b + kk * 2048, C::HALF_BYTES), id_pv, m >= NT || kk > 0);
+          okay = mbar_wait(&p_ready[n & 1], (n >> 1) & 1, kTimeout) && *s_fail == 0;
+          if (!okay) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = kTile / 32; kk < kTile / 16; ++kk)
+            mma_ts(d, a + kk * 8, desc_n_sw128(b + kk * 2048, C::HALF_BYTES), id_pv, 1u);
           mma_commit(&o_done[tile]);
           if (tile == NT - 1) mma_commit(&v_empty[st]);
           if (m + 2 < steps) okay = qk(m + 2);
@@ -376,53 +464,59 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     const uint32_t lanes = (uint32_t)(wq * 32) << 16;
     const int row0 = rblk * C::ROWS + tile * 128 + wq * 32;  // first row of this warp
     const int r = row0 + lane;
-    const int t_row = r / args.group, g_row = r - t_row * args.group;
-    // negative scales become a sign of q; a zero scale a tiny one (masked scores are -inf: not times 0)
-    const bool neg = p.scale < 0.f;
+    const int t_row = token_of(r, args.group_inv), g_row = r - t_row * args.group;
+    // a negative scale negates Q K^T in the MMA; a zero scale is a tiny one (masked scores are -inf: not times 0)
     const float c = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
     uint8_t* myQ = sQ + tile * C::TILE_BYTES;
-    auto stage_q = [&](const Segment& s) {  // this warp's 32 rows, 128-byte-swizzled K-major; missing rows are zeros
+    // this warp's 32 rows, 128-byte-swizzled K-major, missing rows as zeros: asynchronous, q_staged() ends it
+    auto stage_q = [&](const Segment& s) {
       constexpr int CH = D / 8;
-      const int tl = seq_len(p, s.b).tl;
-      const T* q = reinterpret_cast<const T*>(p.q) + s.b * p.q_sb;
-#pragma unroll 4
+      const int tl = lens.at(p, s.b).tl, ch = lane % CH;
+      const T* q = reinterpret_cast<const T*>(p.q) + s.b * p.q_sb + (long long)s.kvh * args.group * p.q_sh + ch * 8;
+#pragma unroll
       for (int it = 0; it < CH; ++it) {
-        const int idx = it * 32 + lane, rr = idx / CH, ch = idx % CH;
-        const int row = row0 + rr, t = row / args.group, g = row - t * args.group;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (t < tl) {
-          v = ld_nc_v4(q + t * p.q_st + (long long)(s.kvh * args.group + g) * p.q_sh + ch * 8);
-          if (neg) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
-        }
-        const int tr = wq * 32 + rr;
-        *reinterpret_cast<uint4*>(myQ + (ch / 8) * C::HALF_BYTES + tr * 128 + (((ch % 8) ^ (tr & 7)) << 4)) = v;
+        const int tr = wq * 32 + (it * 32 + lane) / CH;
+        const int row = rblk * C::ROWS + tile * 128 + tr, t = token_of(row, args.group_inv), g = row - t * args.group;
+        const T* src = q + t * p.q_st + g * p.q_sh;
+        cp_async16_or_zero(myQ + (ch / 8) * C::HALF_BYTES + tr * 128 + (((ch % 8) ^ (tr & 7)) << 4), t < tl ? src : q, t < tl);
       }
+    };
+    auto q_staged = [&]() {
+      asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_ready[tile]);
     };
     int n0 = 0, i0 = 0;
     bool okay = true, have = walk.next(sg);
-    if (have) stage_q(sg);
+    if (have) {
+      stage_q(sg);
+      q_staged();
+    }
     while (have && okay) {
-      const SeqLen sl = seq_len(p, sg.b);
+      const Segment cur = sg;
+      const SeqLen sl = lens.at(p, cur.b);
       const bool live = t_row < sl.tl;
-      const bool warp_live = row0 / args.group < sl.tl;
+      const bool warp_live = token_of(row0, args.group_inv) < sl.tl;
       unsigned long long bits = 0ull;
       if (live) {
-        bits = p.mask ? (unsigned long long)p.mask[sg.b * p.mask_sb + t_row] : (t_row < 63 ? (2ull << t_row) - 1ull : ~0ull);
+        bits = p.mask ? (unsigned long long)p.mask[cur.b * p.mask_sb + t_row] : (t_row < 63 ? (2ull << t_row) - 1ull : ~0ull);
         const int nodes = sl.len - sl.ctx;  // drafted tokens that have a slot
         if (nodes < 64) bits &= (1ull << nodes) - 1ull;
       }
       float m = -INFINITY, l = 0.f;
-      for (int t = sg.t0; t < sg.t1; ++t) {
-        const int j = t - sg.t0, n = n0 + (NT == 1 ? j : 2 * j + tile), i = i0 + j;
+      for (int t = cur.t0; t < cur.t1; ++t) {
+        const int j = t - cur.t0, n = n0 + (NT == 1 ? j : 2 * j + tile), i = i0 + j;
         const uint32_t sbuf = tmem + lanes + ((n & 1) ? C::S1 : C::S0), obuf = tmem + lanes + C::O0 + tile * D;
         const int s0 = t * kTile;
         const bool tail = s0 + kTile > sl.ctx;
         okay = warp_wait(&s_full[n & 1], (n >> 1) & 1, s_fail);
         if (!okay) break;
         tc_fence_after();
+        if (t + 1 == cur.t1) {  // every Q K^T of this piece has completed: the next piece's queries may be staged
+          have = walk.next(sg);
+          if (have) stage_q(sg);
+        }
         if (tail && tile == 0) {
           // thread = slot of the V tile: zero it past the last token, and zero non-finite components of drafted tokens
           const int st = i % C::VS, slot = s0 + (int)threadIdx.x;
@@ -431,27 +525,25 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
           if (slot >= sl.ctx) {
             uint8_t* vr = sV + st * C::TILE_BYTES + threadIdx.x * 128;
 #pragma unroll
-            for (int h = 0; h < C::HALVES; ++h)
+            for (int h = 0; h < C::HALVES; ++h) {
+              uint4 v[8];
+              auto cell = [&](int k) { return reinterpret_cast<uint4*>(vr + h * C::HALF_BYTES + (((k + lane) & 7) << 4)); };
+              if (slot >= sl.len) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                uint4* cell = reinterpret_cast<uint4*>(vr + h * C::HALF_BYTES + (((k + lane) & 7) << 4));
-                if (slot >= sl.len) {
-                  *cell = make_uint4(0, 0, 0, 0);
-                } else {
-                  uint4 v = *cell;
-                  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-                  bool odd = false;
+                for (int k = 0; k < 8; ++k) *cell(k) = make_uint4(0, 0, 0, 0);
+              } else {
+                uint32_t odd = 0;
 #pragma unroll
-                  for (int x = 0; x < 4; ++x) {
-                    if ((w[x] & kExpMask<T>) == kExpMask<T>) w[x] &= 0xFFFF0000u, odd = true;
-                    if (((w[x] >> 16) & kExpMask<T>) == kExpMask<T>) w[x] &= 0x0000FFFFu, odd = true;
-                  }
-                  if (odd) {
-                    *cell = v;
-                    *s_odd = 1;
-                  }
+                for (int k = 0; k < 8; ++k) v[k] = *cell(k);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) odd |= drop_odd<T>(v[k]);
+                if (odd) {
+#pragma unroll
+                  for (int k = 0; k < 8; ++k) *cell(k) = v[k];
+                  *s_odd = 1;
                 }
               }
+            }
           }
           fence_proxy_async();
         }
@@ -474,14 +566,20 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
                 if (!((see >> x) & 1u)) s[k][x] = 0xff800000u;
             }
           }
-          float mx[4];
+          float mx[8];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            mx[k] = __uint_as_float(s[k][0]);
+            auto f = [&](int x) { return __uint_as_float(s[k][x]); };
+            mx[2 * k] = max3(f(0), f(1), f(2));
+            mx[2 * k + 1] = max3(f(16), f(17), f(18));
 #pragma unroll
-            for (int x = 1; x < 32; ++x) mx[k] = fmaxf(mx[k], __uint_as_float(s[k][x]));
+            for (int x = 3; x < 15; x += 2) {
+              mx[2 * k] = max3(mx[2 * k], f(x), f(x + 1));
+              mx[2 * k + 1] = max3(mx[2 * k + 1], f(16 + x), f(17 + x));
+            }
+            mx[2 * k] = max3(mx[2 * k], f(15), f(31));
           }
-          const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+          const float mn = fmaxf(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), mx[6]), fmaxf(mx[7], m));
           if (j == 0) {
             m = mn;
           } else if (__any_sync(0xffffffffu, (mn - m) * c > 8.f)) {
@@ -503,37 +601,45 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
             }
           }
           const float mu = m == -INFINITY ? 0.f : m * c;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t c2 = pair(c, c), mu2 = pair(-mu, -mu);
+          uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             uint32_t w[32];
 #pragma unroll
             for (int x = 0; x < 32; ++x) {
               const int e = 2 * x;  // column 64 k + e
-              const float a = ex2(fmaf(__uint_as_float(s[2 * k + e / 32][e % 32]), c, -mu));
-              const float b = ex2(fmaf(__uint_as_float(s[2 * k + e / 32][e % 32 + 1]), c, -mu));
-              sum[x & 1] += a;
-              sum[2 + (x & 1)] += b;
+              float a, b;
+              unpair(fma2(pair(__uint_as_float(s[2 * k + e / 32][e % 32]), __uint_as_float(s[2 * k + e / 32][e % 32 + 1])), c2, mu2), a, b);
+              a = ex2(a);
+              b = ex2(b);
+              sum[x & 1] = add2(sum[x & 1], pair(a, b));
               w[x] = pack2<T>(a, b);
             }
+            if (k == 0 && j > 0) {  // the previous P V has long ended; seeing its phase keeps this warp's parity in step
+              okay = warp_wait(&o_done[tile], (i - 1) & 1, s_fail);
+              if (!okay) break;
+            }
             tmem_st32(sbuf + 32 * k, w);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(k ? &p_ready[n & 1] : &p_low[n & 1]);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_wait_st();
-        }
-        if (j > 0) {  // the previous P V has long ended; seeing its phase keeps this warp's parity in step
-          okay = warp_wait(&o_done[tile], (i - 1) & 1, s_fail);
           if (!okay) break;
+          float a, b;
+          unpair(add2(sum[0], sum[1]), a, b);
+          l += a + b;
+        } else {
+          if (j > 0) {
+            okay = warp_wait(&o_done[tile], (i - 1) & 1, s_fail);
+            if (!okay) break;
+          }
+          if (lane == 0) mbar_arrive(&p_low[n & 1]), mbar_arrive(&p_ready[n & 1]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[n & 1]);
       }
       if (!okay) break;
-      // every Q K^T of this segment has completed: the next segment's queries may be staged
-      Segment cur = sg;
-      have = walk.next(sg);
-      if (have) stage_q(sg);
+      if (have) q_staged();
       const int tiles = cur.t1 - cur.t0, last = i0 + tiles - 1;
       okay = warp_wait(&o_done[tile], last & 1, s_fail);
       if (!okay) break;
@@ -542,9 +648,11 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
       i0 += tiles;
       const bool whole = tiles == cur.nt;
       const bool odd = *reinterpret_cast<volatile int*>(s_odd) != 0;  // (kept set: a re-check, not a result)
-      const size_t slot = ((size_t)blockIdx.x * 2 + (cur.first ? 0 : 1)) * C::ROWS + tile * 128 + wq * 32 + lane;
-      float* po = args.part_o + slot * D;
-      T* out = reinterpret_cast<T*>(p.out) + cur.b * p.o_sb + t_row * p.o_st + (long long)(cur.kvh * args.group + g_row) * p.o_sh;
+      // partials of a slot: [D / 4][ROWS] vectors of 4 components, and [ROWS] pairs (maximum, sum)
+      const size_t slot = (size_t)blockIdx.x * 2 + (cur.first ? 0 : 1);
+      const int prow = tile * 128 + wq * 32 + lane;
+      uint4* po = reinterpret_cast<uint4*>(args.part_o + slot * C::ROWS * D) + prow;
+      T* out = reinterpret_cast<T*>(p.out) + cur.b * p.o_sb + (long long)cur.kvh * args.group * p.o_sh;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       if (warp_live) {
         const uint32_t obuf = tmem + lanes + C::O0 + tile * D;
@@ -567,40 +675,45 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
               }
             }
           }
-          if (live && whole) {
+          if (whole) {
+            // four lanes trade their rows' vectors, so that each stores 16 of 64 contiguous bytes
+            uint4 v[4];
 #pragma unroll
-            for (int x = 0; x < 32; x += 8) {
+            for (int x = 0; x < 4; ++x) {
               float f[8];
 #pragma unroll
-              for (int y = 0; y < 8; ++y) f[y] = l == 0.f ? 0.f : __uint_as_float(o[x + y]) * inv;
-              *reinterpret_cast<uint4*>(out + 32 * k + x) = Vec<T>::from_float(f);
+              for (int y = 0; y < 8; ++y) f[y] = l == 0.f ? 0.f : __uint_as_float(o[8 * x + y]) * inv;
+              v[x] = Vec<T>::from_float(f);
+            }
+            quad_transpose(v, lane);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int row = row0 + (lane & ~3) + x, t = token_of(row, args.group_inv), g = row - t * args.group;
+              if (t < sl.tl) *reinterpret_cast<uint4*>(out + t * p.o_st + g * p.o_sh + 32 * k + (lane & 3) * 8) = v[x];
             }
           } else if (live) {
 #pragma unroll
-            for (int x = 0; x < 32; x += 4)
-              *reinterpret_cast<uint4*>(po + 32 * k + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+            for (int x = 0; x < 8; ++x)
+              po[(size_t)(8 * k + x) * C::ROWS] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
           }
         }
-        if (live && !whole) {
-          args.part_ml[slot * 2] = m == -INFINITY ? -INFINITY : m * c;
-          args.part_ml[slot * 2 + 1] = l;
-        }
+        if (live && !whole)
+          reinterpret_cast<float2*>(args.part_ml)[slot * C::ROWS + prow] = make_float2(m == -INFINITY ? -INFINITY : m * c, l);
       }
       tc_fence_before();
     }
     if (!okay) {
       // a wait gave up: what this CTA still owed reads as NaN
       const float nan = __uint_as_float(0x7fc00000u);
-      Walk again{cum, p.batch, p.nkv, beg, beg, end};
+      Walk again{lens.cum, p.batch, p.nkv, beg, beg, end};
       while (again.next(sg)) {
-        if (t_row >= seq_len(p, sg.b).tl) continue;
+        if (t_row >= lens.at(p, sg.b).tl) continue;
         if (sg.t1 - sg.t0 == sg.nt) {
           T* out = reinterpret_cast<T*>(p.out) + sg.b * p.o_sb + t_row * p.o_st + (long long)(sg.kvh * args.group + g_row) * p.o_sh;
           for (int d = 0; d < D; ++d) out[d] = from_f<T>(nan);
         } else {
           const size_t slot = ((size_t)blockIdx.x * 2 + (sg.first ? 0 : 1)) * C::ROWS + tile * 128 + wq * 32 + lane;
-          args.part_ml[slot * 2] = 0.f;
-          args.part_ml[slot * 2 + 1] = nan;
+          reinterpret_cast<float2*>(args.part_ml)[slot] = make_float2(0.f, nan);
         }
       }
     }
@@ -613,60 +726,85 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
   }
 }
 
-// Joins the partials of (sequence, head) rows that were cut between shares, one warp per row, in the shares' order:
-// M = max m_i, out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
+// Joins the partials of (sequence, head) rows that were cut between shares, in the shares' order:
+// M = max m_i, out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i. A lane holds one row and 16 of its components, so
+// that the partials' vectors are read 512 bytes at a time and a row is written by whole sectors.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(128) k_tree_join(const __grid_constant__ TreeArgs args) {
   using C = Geo<D, NT>;
-  constexpr int E = D / 32;
+  constexpr int PARTS = D / 16, kBatch = 4;
   const TreeAttnParams& p = args.p;
-  pdl_wait_then_trigger();
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (row >= (long long)p.batch * p.tree * p.nq) return;
-  const int h = (int)(row % p.nq), t = (int)(row / p.nq % p.tree), b = (int)(row / p.nq / p.tree);
-  const int c0 = args.cum[b], c1 = args.cum[b + 1], total = args.cum[p.batch];
-  if (c1 == c0) return;
-  if (p.tree_lens && t >= p.tree_lens[b]) return;
-  const int nt = (c1 - c0) / p.nkv, kvh = h / args.group, r = t * args.group + (h - kvh * args.group);
-  const int i0 = c0 + kvh * nt, rblk = r / C::ROWS, rr = r - rblk * C::ROWS;
-  const int shares = min(args.shares, total);
-  const int s0 = share_of(i0, total, shares), s1 = share_of(i0 + nt - 1, total, shares);
-  if (s0 == s1) return;  // one share held it whole and wrote it
-  auto slot = [&](int s) {
-    const int first = s > s0 || share_beg(s, total, shares) == i0 ? 0 : 1;
-    return ((size_t)(s * args.rb + rblk) * 2 + first) * C::ROWS + rr;
-  };
-  float M = -INFINITY;
-  for (int s = s0 + lane; s <= s1; s += 32) M = fmaxf(M, args.part_ml[slot(s) * 2]);
-  M = warp_max(M);
-  float L = 0.f, o[E];
+  const int b = blockIdx.z, kvh = blockIdx.y;
+  const int unit = (int)blockIdx.x * 4 + (threadIdx.x >> 5), part = unit % PARTS, r = unit / PARTS * 32 + lane;
+  const int t = token_of(r, args.group_inv), g = r - t * args.group;
+  const int rblk = r / C::ROWS, rr = r - rblk * C::ROWS;
+  // the lengths were complete before the attention started (it waited for its predecessor before it let this kernel
+  // start), so the arithmetic on them runs beside the attention
+  __shared__ int mem[3 * kMaxBatch + 1];
+  Lens lens(mem);
+  lens.fill(p);
+  const int c0 = lens.cum[b], c1 = lens.cum[b + 1], total = lens.cum[p.batch];
+  const bool live = c1 > c0 && t < lens.at(p, b).tl;
+  const int cost = (c1 - c0) / p.nkv, nt = cost - kPieceCost, at = c0 + kvh * cost, i0 = at + kPieceCost;
+  const int shares = max(1, min(args.shares, total));
+  const int s0 = live ? share_of(i0, total, shares) : 0, s1 = live ? share_of(i0 + nt - 1, total, shares) : 0;
+  pdl_wait_then_trigger();  // by every thread: what follows this kernel in the stream counts on the attention's end
+  if (s0 == s1) return;     // one share held it whole and wrote it
+  const int first = share_beg(s0, total, shares) >= at ? 0 : 1;
+  auto slot = [&](int s) { return (size_t)(s * args.rb + rblk) * 2 + (s == s0 ? first : 0); };
+  const float2* ml = reinterpret_cast<const float2*>(args.part_ml) + rr;
+  const float4* po = reinterpret_cast<const float4*>(args.part_o) + (size_t)part * 4 * C::ROWS + rr;
+  float M = -INFINITY, L = 0.f;
+  float4 o[4];
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int s = s0; s <= s1; ++s) {
-    const size_t k = slot(s);
-    const float2 ml = *reinterpret_cast<const float2*>(args.part_ml + k * 2);
-    if (ml.x == -INFINITY) continue;
-    const float f = exp2f(ml.x - M);
-    L += f * ml.y;
-    float v[E];
-    if constexpr (E == 4)
-      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(args.part_o + k * D + lane * E);
-    else
-      *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(args.part_o + k * D + lane * E);
+  for (int x = 0; x < 4; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int q0 = s0; q0 <= s1; q0 += kBatch) {  // kBatch shares' loads in flight together
+    float2 e[kBatch];
+    float4 v[kBatch][4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += f * v[e];
+    for (int q = 0; q < kBatch; ++q) {
+      e[q] = make_float2(-INFINITY, 0.f);
+      if (q0 + q <= s1) {
+        const size_t k = slot(q0 + q) * C::ROWS;
+        e[q] = ml[k];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[q][x] = po[k * (D / 4) + x * C::ROWS];
+      }
+    }
+    float mn = M;
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) mn = fmaxf(mn, e[q].x);
+    if (mn > M) {
+      const float f = exp2f(M - mn);
+      M = mn;
+      L *= f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[x].x *= f, o[x].y *= f, o[x].z *= f, o[x].w *= f;
+    }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+      if (e[q].x != -INFINITY) {  // (a piece in which the row sees nothing, or no piece)
+        const float f = exp2f(e[q].x - M);
+        L += f * e[q].y;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          o[x].x += f * v[q][x].x;
+          o[x].y += f * v[q][x].y;
+          o[x].z += f * v[q][x].z;
+          o[x].w += f * v[q][x].w;
+        }
+      }
   }
-  T* out = reinterpret_cast<T*>(p.out) + b * p.o_sb + t * p.o_st + h * p.o_sh + lane * E;
+  T* out = reinterpret_cast<T*>(p.out) + b * p.o_sb + t * p.o_st + (long long)(kvh * args.group + g) * p.o_sh + part * 16;
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  uint32_t w[E / 2];
 #pragma unroll
-  for (int e = 0; e < E; e += 2) w[e / 2] = L == 0.f ? 0u : pack2<T>(o[e] * inv, o[e + 1] * inv);
-  if constexpr (E == 4)
-    *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
-  else
-    *reinterpret_cast<uint32_t*>(out) = w[0];
+  for (int x = 0; x < 2; ++x) {
+    float f[8] = {o[2 * x].x, o[2 * x].y, o[2 * x].z, o[2 * x].w, o[2 * x + 1].x, o[2 * x + 1].y, o[2 * x + 1].z, o[2 * x + 1].w};
+#pragma unroll
+    for (int y = 0; y < 8; ++y) f[y] = L == 0.f ? 0.f : f[y] * inv;
+    reinterpret_cast<uint4*>(out)[x] = Vec<T>::from_float(f);
+  }
 }
 
 struct Plan {
@@ -681,7 +819,7 @@ Plan plan_of(const TreeAttnParams& p) {
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   pl.max_tiles = (p.max_blocks + kTilePages - 1) / kTilePages;
-  const long long most = (long long)std::min(p.batch, kMaxBatch) * p.nkv * pl.max_tiles;
+  const long long most = (long long)std::min(p.batch, kMaxBatch) * p.nkv * (pl.max_tiles + kPieceCost);
   pl.shares = (int)std::max<long long>(1, std::min<long long>(most, sms / pl.rb));
   return pl;
 }
@@ -698,9 +836,9 @@ cudaError_t launch(TreeArgs a, const Plan& pl, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   e = launch_k(fn, dim3(pl.shares * pl.rb), dim3(C::THREADS), C::SMEM, s, a);
   if (e != cudaSuccess || pl.max_tiles == 1) return e;  // one tile per (sequence, head): nothing is ever cut
-  const long long rows = (long long)a.p.batch * a.p.tree * a.p.nq;
+  const int units = (a.p.tree * a.group + 31) / 32 * (D / 16);  // warps per (sequence, KV head)
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((rows + 3) / 4));
+  cfg.gridDim = dim3((units + 3) / 4, a.p.nkv, a.p.batch);
   cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -714,23 +852,23 @@ cudaError_t launch(TreeArgs a, const Plan& pl, cudaStream_t s) {
 }  // namespace
 
 size_t tree_attention_scratch_bytes(const TreeAttnParams& p) {
-  return (kMaxBatch + 4) * sizeof(int) + part_floats(p, plan_of(p)) * sizeof(float);
+  return part_floats(p, plan_of(p)) * sizeof(float);
 }
 
 cudaError_t tree_attention(const TreeAttnParams& p, void* scratch, cudaStream_t s) {
   if ((p.head_dim != 64 && p.head_dim != 128) || p.batch <= 0 || p.tree <= 0 || p.tree > 64 || p.nkv <= 0 ||
-      p.nq <= 0 || p.nq % p.nkv != 0 || p.max_blocks <= 0 || p.num_blocks <= 0 || (p.dtype != kBF16 && p.dtype != kF16))
+      p.nq <= 0 || p.nq % p.nkv != 0 || p.nkv > 65535 || p.max_blocks <= 0 || p.num_blocks <= 0 || (p.dtype != kBF16 && p.dtype != kF16))
     return cudaErrorInvalidValue;
   const Plan pl = plan_of(p);
-  if (pl.rb > 148 || (long long)std::min(p.batch, kMaxBatch) * p.nkv * pl.max_tiles >= (1ll << 31)) return cudaErrorInvalidValue;
+  if (pl.rb > 148 || (long long)std::min(p.batch, kMaxBatch) * p.nkv * (pl.max_tiles + kPieceCost) >= (1ll << 31)) return cudaErrorInvalidValue;
   const bool bf16 = p.dtype == kBF16;
   TreeArgs a;
   a.p = p;
   a.group = p.nq / p.nkv;
+  a.group_inv = a.group > 1 ? (uint32_t)(((1ull << 32) + a.group - 1) / a.group) : 0u;
   a.rb = pl.rb;
   a.shares = pl.shares;
-  a.cum = reinterpret_cast<int*>(scratch);
-  a.part_o = reinterpret_cast<float*>(a.cum + kMaxBatch + 4);
+  a.part_o = reinterpret_cast<float*>(scratch);
   a.part_ml = a.part_o + (size_t)pl.shares * pl.rb * 2 * pl.nt * 128 * p.head_dim;
   const uint64_t rows = (uint64_t)p.num_blocks * p.nkv * kPage;
   cudaError_t e = tensor_map_2d(p.k_cache, rows, p.head_dim, p.head_dim * 2, kPage, 64, bf16, &a.tk);

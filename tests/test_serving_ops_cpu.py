@@ -107,54 +107,55 @@ def test_host_tensors_are_refused():
                                    torch.zeros(1, 1, 1, 8), torch.zeros(1, 1, 16, 8), torch.zeros(1, 1, 16, 8), 1, 1)
 
 
-def _shares(total, shares):
-    return [(c * total // shares, (c + 1) * total // shares) for c in range(shares)]
-
-
 @pytest.mark.parametrize("most", [1, 7, 49, 74, 148])
 def test_tree_attention_shares_cover_once_and_join_what_was_cut(most):
-    """csrc/tree_attention.cu's partition: every (sequence, KV head, tile) belongs to one share, a share's pieces of a
-    cut (sequence, head) sit in slot 0 (piece starts the share) or 1, and the joining kernel's arithmetic finds exactly
-    these slots, in order."""
-    for nkv, tiles in [(1, [1]), (8, [9]), (2, [3, 0, 5, 1]), (8, [17] * 8), (1, [0, 0, 4]), (4, list(range(13))), (8, [257, 1, 30])]:
+    """csrc/tree_attention.cu's partition: positions are COST per (sequence, KV head) plus one per tile; every tile
+    belongs to one share, a share's pieces of a cut (sequence, head) sit in slot 0 (the piece's head holds the share's
+    first position) or 1, and the joining kernel's arithmetic finds exactly these slots, in order."""
+    COST = 2
+    for nkv, tiles in [(1, [1]), (8, [9]), (2, [3, 0, 5, 1]), (8, [17] * 8), (1, [0, 0, 4]), (4, list(range(13))), (8, [257, 1, 30]),
+                       (3, [1] * 40), (1, [400])]:
         cum = [0]
         for t in tiles:
-            cum.append(cum[-1] + t * nkv)
+            cum.append(cum[-1] + ((t + COST) * nkv if t else 0))
         total = cum[-1]
         shares = min(most, total)
         written, seen = {}, set()
-        for c, (beg, end) in enumerate(_shares(total, shares)):
+        for c in range(shares):
+            beg, end = c * total // shares, (c + 1) * total // shares
+            assert beg < end
             g = beg
             while g < end:
                 b = max(i for i in range(len(tiles)) if cum[i] <= g)
-                nt = (cum[b + 1] - cum[b]) // nkv
-                kvh, t0 = (g - cum[b]) // nt, (g - cum[b]) % nt
-                t1 = min(nt, t0 + end - g)
+                cost = (cum[b + 1] - cum[b]) // nkv
+                rem = g - cum[b]
+                kvh, nt = rem // cost, cost - COST
+                at = g - (rem - kvh * cost)
+                t0, t1 = max(0, g - at - COST), min(nt, end - at - COST)
+                first, g = g == beg, min(end, at + cost)
+                if t0 >= t1:
+                    continue
                 for t in range(t0, t1):
                     assert (b, kvh, t) not in seen
                     seen.add((b, kvh, t))
                 if t1 - t0 < nt:
-                    key = (c, 0 if g == beg else 1)
+                    key = (c, 0 if first else 1)
                     assert key not in written
                     written[key] = (b, kvh, t0)
-                g += t1 - t0
-        assert len(seen) == total
+        assert len(seen) == nkv * sum(tiles)
         joined = set()
+
+        def share_of(g):
+            return ((g + 1) * shares - 1) // total
+
         for b, nt in enumerate(tiles):
             for kvh in range(nkv if nt else 0):
-                i0 = cum[b] + kvh * nt
-
-                def share_of(g):
-                    return ((g + 1) * shares - 1) // total
-
-                s0, s1 = share_of(i0), share_of(i0 + nt - 1)
-                at = -1
+                at = cum[b] + kvh * (nt + COST)
+                s0, s1 = share_of(at + COST), share_of(at + COST + nt - 1)
+                last = -1
                 for s in range(s0, s1 + 1) if s0 != s1 else ():
-                    beg, end = s * total // shares, (s + 1) * total // shares
-                    key = (s, 0 if s > s0 or beg == i0 else 1)
-                    if beg == end:
-                        raise AssertionError("an empty share between a row's shares")
-                    assert written[key][:2] == (b, kvh) and written[key][2] > at
-                    at = written[key][2]
+                    key = (s, 0 if s > s0 or s * total // shares >= at else 1)
+                    assert written[key][:2] == (b, kvh) and written[key][2] > last
+                    last = written[key][2]
                     joined.add(key)
         assert joined == set(written)

@@ -13,8 +13,10 @@
 // and the interleaved layout, hold vectors 2s and 2s + 1. No shuffles but the norm's sum. Statistics, products
 // and sums are fp32; every output is rounded once, at its store.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
+#include "packed.cuh"
 #include "serve_ops.h"
 
 namespace cob {
@@ -22,6 +24,23 @@ namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kPage = 16;  // tokens per cache page
+
+// two 16-bit components of a word
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));  // bf16: the upper half of an fp32
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
 
 // V components of T as one load
 template <typename T, int V>
@@ -46,11 +65,14 @@ struct Pack {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < V; ++i) f[i] = __uint_as_float(w[i]);
+    } else if constexpr (V == 1) {
+      const uint16_t h = (uint16_t)w[0];
+      f[0] = to_f(*reinterpret_cast<const T*>(&h));
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-        f[i] = to_f(*reinterpret_cast<const T*>(&h));
+      for (int i = 0; i < kWords; ++i) {
+        const float2 t = unpack2<T>(w[i]);
+        f[2 * i] = t.x, f[2 * i + 1] = t.y;
       }
     }
   }
@@ -58,16 +80,12 @@ struct Pack {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < V; ++i) w[i] = __float_as_uint(f[i]);
+    } else if constexpr (V == 1) {
+      const T t = from_f<T>(f[0]);
+      w[0] = *reinterpret_cast<const uint16_t*>(&t);
     } else {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) {
-        const T lo = from_f<T>(f[2 * i]);
-        w[i] = *reinterpret_cast<const uint16_t*>(&lo);
-        if constexpr (V > 1) {
-          const T hi = from_f<T>(f[2 * i + 1]);
-          w[i] |= (uint32_t) * reinterpret_cast<const uint16_t*>(&hi) << 16;
-        }
-      }
+      for (int i = 0; i < kWords; ++i) w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
     }
   }
   __device__ __forceinline__ void store(T* p) const {
@@ -82,20 +100,19 @@ struct Pack {
   }
 };
 
-// what a lane needs of its slots: component offsets of the two vectors, and which pairs rotate
+// what a lane needs of one of its slots
 template <int V>
 struct Slot {
-  int a, b;     // first component of each vector
-  int j;        // first pair index (into the tables)
-  bool on;      // slot exists
+  int a, b;  // first component of each vector
+  int j;     // first rotation pair (index into the tables)
+  bool on;   // the slot exists
 };
-template <int V>
-__device__ __forceinline__ Slot<V> slot_of(int s, int nslots, int rot, int interleaved) {
+template <int V, bool INTER>
+__device__ __forceinline__ Slot<V> slot_of(int s, int nslots, int half) {
   Slot<V> r;
   r.on = s < nslots;
   r.j = s * V;
-  const int half = rot / 2;
-  if (!interleaved && r.j < half) {
+  if (!INTER && r.j < half) {
     r.a = r.j;
     r.b = r.j + half;
   } else {
@@ -105,187 +122,260 @@ __device__ __forceinline__ Slot<V> slot_of(int s, int nslots, int rot, int inter
   return r;
 }
 
-// cos / sin of the lane's pairs at one table row; pairs past rot / 2 do not rotate
-template <int V>
-__device__ __forceinline__ void load_angles(const float* ct, const float* st, size_t row, int j, int half, bool on,
-                                            float* c, float* sn) {
-  if (on && V % 4 == 0 && half % 4 == 0 && j + V <= half) {
-#pragma unroll
-    for (int i = 0; i + 3 < V; i += 4) {
-      const float4 cv = __ldg(reinterpret_cast<const float4*>(ct + row * half + j + i));
-      const float4 sv = __ldg(reinterpret_cast<const float4*>(st + row * half + j + i));
-      c[i] = cv.x, c[i + 1] = cv.y, c[i + 2] = cv.z, c[i + 3] = cv.w;
-      sn[i] = sv.x, sn[i + 1] = sv.y, sn[i + 2] = sv.z, sn[i + 3] = sv.w;
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const bool r = on && j + i < half;
-    c[i] = r ? __ldg(ct + row * half + j + i) : 1.f;
-    sn[i] = r ? __ldg(st + row * half + j + i) : 0.f;
-  }
-}
-
-// (a, b) turned by the angle of (c, s); the roundings are spelled out, so that every variant gives the same bits
-__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
-  const float x = a, y = b;
-  a = __fmaf_rn(x, c, -__fmul_rn(y, s));
-  b = __fmaf_rn(y, c, __fmul_rn(x, s));
-}
-
-// rotate a slot's 2 V components in place; components past `half` pairs pass through untouched (not as x * 1 -
-// y * 0, which an infinity next to them would turn into NaN)
-template <int V>
-__device__ __forceinline__ void rotate(float* x, const float* c, const float* sn, int j, int half, int interleaved) {
-  if (!interleaved) {
-    if (j < half) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) turn(x[i], x[V + i], c[i], sn[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (j + i < half) turn(x[2 * i], x[2 * i + 1], c[i], sn[i]);
-  }
-}
-
+// V weights (fp32 or T) from component `off`, a multiple of V (the launcher's vectors fit the weights' alignment too)
 template <typename T, int V>
 __device__ __forceinline__ void load_weights(const void* w, int f32, int off, float* o) {
+  if (f32) {
+    constexpr int N = V < 4 ? V : 4;
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    o[i] = f32 ? __ldg(reinterpret_cast<const float*>(w) + off + i) : to_f(__ldg(reinterpret_cast<const T*>(w) + off + i));
+    for (int i = 0; i < V; i += N) {
+      Pack<float, N> r;
+      r.load(reinterpret_cast<const float*>(w) + off + i);
+      r.to_float(o + i);
+    }
+  } else {
+    Pack<T, V> r;
+    r.load(reinterpret_cast<const T*>(w) + off);
+    r.to_float(o);
+  }
 }
+
+// A slot's 2 V components in fp32 as V register pairs: pair k holds components 2k, 2k + 1 of (first vector, second
+// vector). `within`: the two components of a pair turn with each other (interleaved layout, and V = 1); otherwise pair k
+// of the first vector turns with pair k of the second.
+template <typename T, int V>
+__device__ __forceinline__ void to_pairs(const Pack<T, V>& lo, const Pack<T, V>& hi, uint64_t* x) {
+  float f[2 * V];
+  lo.to_float(f);
+  hi.to_float(f + V);
+#pragma unroll
+  for (int k = 0; k < V; ++k) x[k] = pair(f[2 * k], f[2 * k + 1]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_zeros(T* lo, T* hi) {
+  Pack<T, V> o;
+#pragma unroll
+  for (int i = 0; i < Pack<T, V>::kWords; ++i) o.w[i] = 0;
+  o.store(lo);
+  o.store(hi);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pairs(const uint64_t* x, T* lo, T* hi) {
+  float f[2 * V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) unpair(x[k], f[2 * k], f[2 * k + 1]);
+  Pack<T, V> o;
+  o.from_float(f);
+  o.store(lo);
+  o.from_float(f + V);
+  o.store(hi);
+}
+
+// What turns a slot by one position's angles: pair k becomes x c + mate(x) s, with the rotation's signs in s and, where
+// weights are given, each coefficient times the weight of the component that it multiplies. Pairs past the rotary part get
+// c = 1 (or the weight) and are only multiplied.
+template <int V, bool INTER>
+struct Turn {
+  static constexpr bool kWithin = INTER || V == 1;
+  uint64_t c[V], s[V];
+  __device__ __forceinline__ void load(const float* ct, const float* st, size_t row, int j, int half, bool on, float sign,
+                                       const float* w) {
+    float cv[V], sv[V];
+    ct += row * half + j;
+    st += row * half + j;
+    if (on && V % 4 == 0 && half % 4 == 0 && j + V <= half) {
+#pragma unroll
+      for (int i = 0; i + 3 < V; i += 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(ct + i)), b = __ldg(reinterpret_cast<const float4*>(st + i));
+        cv[i] = a.x, cv[i + 1] = a.y, cv[i + 2] = a.z, cv[i + 3] = a.w;
+        sv[i] = b.x, sv[i + 1] = b.y, sv[i + 2] = b.z, sv[i + 3] = b.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const bool turns = on && j + i < half;
+        cv[i] = turns ? __ldg(ct + i) : 1.f;
+        sv[i] = turns ? __ldg(st + i) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      float a[2], b[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int e = 2 * k + h, m = kWithin ? e ^ 1 : (e < V ? e + V : e - V);  // component and its mate
+        const int at = kWithin ? k : e % V;                                     // their angle
+        const bool second = kWithin ? h == 1 : e >= V;
+        a[h] = w ? cv[at] * w[e] : cv[at];
+        b[h] = second ? sv[at] * sign : sv[at] * -sign;
+        if (w) b[h] *= w[m];
+      }
+      c[k] = pair(a[0], a[1]);
+      s[k] = pair(b[0], b[1]);
+    }
+  }
+  // the roundings are those of fma(x, c, mate * s) in every variant; what does not rotate is not x c + mate 0, which an
+  // infinity in the mate would turn into NaN
+  __device__ __forceinline__ void apply(uint64_t* x, int j, int half, bool weighted) const {
+    if (INTER ? j + V <= half : j < half) {
+      uint64_t y[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) y[k] = mul2(mate(x, k), s[k]);
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[k] = fma2(x[k], c[k], y[k]);
+    } else if (INTER && j < half) {  // the rotary part ends inside the slot
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[k] = j + k < half ? fma2(x[k], c[k], mul2(mate(x, k), s[k])) : mul2(x[k], c[k]);
+    } else if (weighted) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[k] = mul2(x[k], c[k]);
+    }
+  }
+  static __device__ __forceinline__ uint64_t mate(const uint64_t* x, int k) {
+    if constexpr (kWithin) {
+      float a, b;
+      unpair(x[k], a, b);
+      return pair(b, a);
+    } else {
+      return x[k < V / 2 ? k + V / 2 : k - V / 2];
+    }
+  }
+};
 
 __device__ __forceinline__ float group_sum(float v, int gl) {
   for (int o = gl >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
+// What a kernel is compiled for: kAnything decides at run time (the narrow-vector forms)
+enum Mode : int { kPlain = 0, kNorm = 1, kAppend = 2, kAppendNorm = 3, kAnything = 4 };
+
 struct RotaryArgs {
   RotaryParams p;
-  int gl;          // lanes per head
-  int hb;          // heads per warp and step
-  int blocks[3];   // head blocks of q, k, v per row
+  int gl, gl_shift;  // lanes per head
+  int hb;            // heads per warp
+  int blocks[3];     // head blocks of q, k, v per row
+  int wh_shift;      // log2 of the warps of a block side by side on one row's head blocks (they share its angles in L1)
+  uint32_t seq_inv;  // ceil(2^32 / seq): row / seq = high word of row * seq_inv; 0: divide
 };
+__device__ __forceinline__ int batch_of(int row, int seq, uint32_t inv) {
+  return inv ? (int)__umulhi((uint32_t)row, inv) : row / seq;
+}
 
 // One warp takes `hb` heads of one row: 32 / gl heads side by side, HPT after one another with all their loads
-// in flight; cos, sin and the weights are loaded once for them.
-template <typename T, int V, int NSL, int HPT>
-__global__ void __launch_bounds__(kThreads) k_rotary(const __grid_constant__ RotaryArgs args) {
+// in flight; the angles and weights are loaded and combined once for them.
+template <typename T, int V, int NSL, int HPT, int MODE, bool INTER>
+__global__ void __launch_bounds__(kThreads, HPT > 1 ? ((MODE & kNorm) ? 4 : 5) : NSL == 1 ? 6 : 1)
+    k_rotary(const __grid_constant__ RotaryArgs args) {
   const RotaryParams& p = args.p;
   pdl_wait_then_trigger();
-  const int hblocks = args.blocks[0] + args.blocks[1] + args.blocks[2];
-  const long long unit = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const long long row = unit / hblocks;
-  if (row >= (long long)p.batch * p.seq) return;
-  int hblk = (int)(unit - row * hblocks), kind = 0;
+  const int warp = threadIdx.x >> 5;
+  const int row = (int)blockIdx.x * (kWarps >> args.wh_shift) + (warp >> args.wh_shift);
+  int hblk = ((int)blockIdx.y << args.wh_shift) + (warp & ((1 << args.wh_shift) - 1)), kind = 0;
+  if (row >= p.batch * p.seq || hblk >= args.blocks[0] + args.blocks[1] + args.blocks[2]) return;
   while (kind < 2 && hblk >= args.blocks[kind]) hblk -= args.blocks[kind++];
-  const int b = (int)(row / p.seq), s = (int)(row - (long long)b * p.seq);
-  const int lane = threadIdx.x & 31, gl = args.gl, l = lane & (gl - 1), sub = lane / gl, per = 32 / gl;
+  const bool append = MODE == kAnything ? p.append != 0 : MODE >= kAppend;
+  const bool norm = kind < 2 && (MODE == kAnything ? p.w[0] != nullptr : (MODE & kNorm) != 0);
+  const bool has_bias = (MODE == kAnything || MODE >= kAppend) && p.bias != nullptr;
+  const int b = batch_of(row, p.seq, args.seq_inv), s = row - b * p.seq;
+  const int lane = threadIdx.x & 31, gl = args.gl, l = lane & (gl - 1), sub = lane >> args.gl_shift, per = 32 >> args.gl_shift;
   const int half = p.rot / 2, nslots = p.D / (2 * V);
   const int pos = p.pos[b * p.pos_sb + s * p.pos_ss];
   const bool in_table = pos >= 0 && pos < p.max_pos;
-  long long cache_row = -1;  // append: (block * nkv) * page + slot within it, in rows of the head's page
-  int page_off = 0;
-  if (p.append) {
-    if (!in_table || (p.lens && s >= p.lens[b])) return;
-    if (kind > 0) {
-      const int start = p.starts[b];
-      const long long slot = (long long)start + s;
-      if (start < 0 || slot >= (long long)p.max_blocks * kPage) return;
-      const int blk = p.block_tables[(size_t)b * p.max_blocks + (int)(slot / kPage)];
-      if (blk < 0 || blk >= p.num_blocks) return;
-      page_off = (int)(slot % kPage);
-      cache_row = (long long)blk * p.in[kind].heads;
-    }
-  }
+  const int start = append && kind > 0 ? p.starts[b] : 0;
+  if (append && (!in_table || (p.lens && s >= p.lens[b]))) return;
   const HeadView& in = p.in[kind];
-  const T* src = reinterpret_cast<const T*>(in.p) + b * in.sb + s * in.ss;
+  const int head0 = hblk * args.hb + sub;  // this lane's first head, then every `per`-th
+  const T* src = reinterpret_cast<const T*>(in.p) + b * in.sb + s * in.ss + head0 * in.sh;
+  const long long src_step = per * in.sh;
   Slot<V> sl[NSL];
   Pack<T, V> raw[HPT][NSL][2];
 #pragma unroll
-  for (int n = 0; n < NSL; ++n) sl[n] = slot_of<V>(l + n * gl, nslots, p.rot, p.interleaved);
+  for (int n = 0; n < NSL; ++n) sl[n] = slot_of<V, INTER>(l + n * gl, nslots, half);
 #pragma unroll
-  for (int h = 0; h < HPT; ++h) {
-    const int head = hblk * args.hb + h * per + sub;
+  for (int h = 0; h < HPT; ++h, src += src_step)
 #pragma unroll
     for (int n = 0; n < NSL; ++n)
-      if (head < in.heads && sl[n].on) {
-        raw[h][n][0].load(src + head * in.sh + sl[n].a);
-        raw[h][n][1].load(src + head * in.sh + sl[n].b);
+      if (head0 + h * per < in.heads && sl[n].on) {
+        raw[h][n][0].load(src + sl[n].a);
+        raw[h][n][1].load(src + sl[n].b);
       }
-  }
-  float c[NSL][V], sn[NSL][V], w[NSL][2 * V];
-  const bool norm = kind < 2 && p.w[0] != nullptr;
+  Turn<V, INTER> turn[NSL];
   if (kind < 2) {
 #pragma unroll
     for (int n = 0; n < NSL; ++n) {
-      load_angles<V>(p.cos_t, p.sin_t, in_table ? pos : 0, sl[n].j, half, sl[n].on, c[n], sn[n]);
-      if (p.inverse) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) sn[n][i] = -sn[n][i];
-      }
+      float w[2 * V];
       if (norm && sl[n].on) {
-        load_weights<T, V>(p.w[kind], p.w_f32, sl[n].a, w[n]);
-        load_weights<T, V>(p.w[kind], p.w_f32, sl[n].b, w[n] + V);
+        load_weights<T, V>(p.w[kind], p.w_f32, sl[n].a, w);
+        load_weights<T, V>(p.w[kind], p.w_f32, sl[n].b, w + V);
       }
+      turn[n].load(p.cos_t, p.sin_t, in_table ? pos : 0, sl[n].j, half, sl[n].on, p.inverse ? -1.f : 1.f, norm ? w : nullptr);
     }
   }
   T* dst;
   long long dst_sh;
-  if (p.append && kind > 0) {
+  if (append && kind > 0) {
+    const long long slot = (long long)start + s;
+    if (start < 0 || slot >= (long long)p.max_blocks * kPage) return;
+    const int blk = p.block_tables[(size_t)b * p.max_blocks + (int)(slot / kPage)];
+    if (blk < 0 || blk >= p.num_blocks) return;
     T* cache = reinterpret_cast<T*>(kind == 1 ? p.k_cache : p.v_cache);
-    dst = cache + (cache_row * kPage + page_off) * p.D;
+    dst = cache + ((long long)blk * in.heads * kPage + slot % kPage) * p.D;
     dst_sh = (long long)kPage * p.D;
   } else {
     const HeadView& o = p.out[kind];
     dst = reinterpret_cast<T*>(const_cast<void*>(o.p)) + b * o.sb + s * o.ss;
     dst_sh = o.sh;
   }
-  const int head0 = (kind > 0 ? p.in[0].heads : 0) + (kind > 1 ? p.in[1].heads : 0);  // bias order: q, k, v
+  dst += head0 * dst_sh;
+  const long long dst_step = per * dst_sh;
+  if (!append && !in_table) {  // a padded row
 #pragma unroll
-  for (int h = 0; h < HPT; ++h) {
-    const int head = hblk * args.hb + h * per + sub;
-    const bool live = head < in.heads;
-    float x[NSL][2 * V], ss = 0.f;
-#pragma unroll
-    for (int n = 0; n < NSL; ++n) {
-      if (live && sl[n].on) {
-        raw[h][n][0].to_float(x[n]);
-        raw[h][n][1].to_float(x[n] + V);
-        if (p.bias) {
-          const T* bp = reinterpret_cast<const T*>(p.bias) + (size_t)(head0 + head) * p.D;
-          float bf[2 * V];
-          load_weights<T, V>(bp, 0, sl[n].a, bf);
-          load_weights<T, V>(bp, 0, sl[n].b, bf + V);
-#pragma unroll
-          for (int i = 0; i < 2 * V; ++i) x[n][i] += bf[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 2 * V; ++i) ss += x[n][i] * x[n][i];
-      }
-    }
-    if (norm) {
-      const float rstd = rsqrtf(group_sum(ss, gl) / (float)p.D + p.eps);
+    for (int h = 0; h < HPT; ++h, dst += dst_step)
 #pragma unroll
       for (int n = 0; n < NSL; ++n)
+        if (head0 + h * per < in.heads && sl[n].on) store_zeros<T, V>(dst + sl[n].a, dst + sl[n].b);
+    return;
+  }
+  // bias order: q, k, v heads
+  const int bias0 = (kind > 0 ? p.in[0].heads : 0) + (kind > 1 ? p.in[1].heads : 0) + head0;
+  const T* bias = reinterpret_cast<const T*>(p.bias) + (size_t)bias0 * p.D;
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) x[n][i] = x[n][i] * rstd * w[n][i];
+  for (int h = 0; h < HPT; ++h, dst += dst_step, bias += per * p.D) {
+    const bool live = head0 + h * per < in.heads;
+    uint64_t x[NSL][V], ss = pair(0.f, 0.f);
+#pragma unroll
+    for (int n = 0; n < NSL; ++n)
+      if (live && sl[n].on) {
+        to_pairs(raw[h][n][0], raw[h][n][1], x[n]);
+        if (has_bias) {
+          Pack<T, V> b0, b1;
+          b0.load(bias + sl[n].a);
+          b1.load(bias + sl[n].b);
+          uint64_t bf[V];
+          to_pairs(b0, b1, bf);
+#pragma unroll
+          for (int k = 0; k < V; ++k) x[n][k] = add2(x[n][k], bf[k]);
+        }
+        if (norm) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) ss = fma2(x[n][k], x[n][k], ss);
+        }
+      }
+    uint64_t rstd = 0;
+    if (norm) {
+      const float r = rsqrtf(group_sum(sum2(ss), gl) / (float)p.D + p.eps);
+      rstd = pair(r, r);
     }
 #pragma unroll
     for (int n = 0; n < NSL; ++n)
       if (live && sl[n].on) {
-        if (kind < 2) rotate<V>(x[n], c[n], sn[n], sl[n].j, half, p.interleaved);
-        if (!in_table) {
+        if (kind < 2) turn[n].apply(x[n], sl[n].j, half, norm);
+        if (norm) {
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) x[n][i] = 0.f;
+          for (int k = 0; k < V; ++k) x[n][k] = mul2(x[n][k], rstd);
         }
-        Pack<T, V> o;
-        o.from_float(x[n]);
-        o.store(dst + head * dst_sh + sl[n].a);
-        o.from_float(x[n] + V);
-        o.store(dst + head * dst_sh + sl[n].b);
+        store_pairs<T, V>(x[n], dst + sl[n].a, dst + sl[n].b);
       }
   }
 }
@@ -295,11 +385,13 @@ __global__ void __launch_bounds__(kThreads) k_rotary(const __grid_constant__ Rot
 // order: thread, lanes of equal slots, warps, blocks (k_weight_grad).
 struct RotaryBwdArgs {
   RotaryParams p;
-  int gl, hb, blocks[2], nb[2];
+  int gl, gl_shift, hb, blocks[2], nb[2];
+  int inner, groups[2];  // head blocks that a warp takes with one load of the angles; groups of them in a row
+  uint32_t seq_inv, groups_inv[2];
   float* ws;  // [nb[0] + nb[1]][D]
 };
 
-template <typename T, int V, int NSL, int HPT>
+template <typename T, int V, int NSL, int HPT, bool INTER>
 __global__ void __launch_bounds__(kThreads) k_rotary_norm_bwd(const __grid_constant__ RotaryBwdArgs args) {
   const RotaryParams& p = args.p;
   extern __shared__ float sdw[];  // [kWarps][D]
@@ -307,100 +399,110 @@ __global__ void __launch_bounds__(kThreads) k_rotary_norm_bwd(const __grid_const
   const int kind = (int)blockIdx.x < args.nb[0] ? 0 : 1;
   const int blk = kind ? (int)blockIdx.x - args.nb[0] : (int)blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int gl = args.gl, l = lane & (gl - 1), sub = lane / gl, per = 32 / gl;
+  const int gl = args.gl, l = lane & (gl - 1), sub = lane >> args.gl_shift, per = 32 >> args.gl_shift;
   const int half = p.rot / 2, nslots = p.D / (2 * V), hblocks = args.blocks[kind];
   const HeadView &in = p.in[kind], &gr = p.grad[kind], &o = p.out[kind];
   Slot<V> sl[NSL];
-  float w[NSL][2 * V], dw[NSL][2 * V];
+  uint64_t w[NSL][V], dw[NSL][V];
 #pragma unroll
   for (int n = 0; n < NSL; ++n) {
-    sl[n] = slot_of<V>(l + n * gl, nslots, p.rot, p.interleaved);
+    sl[n] = slot_of<V, INTER>(l + n * gl, nslots, half);
+    float f[2 * V];
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i) f[i] = 0.f;
     if (sl[n].on) {
-      load_weights<T, V>(p.w[kind], p.w_f32, sl[n].a, w[n]);
-      load_weights<T, V>(p.w[kind], p.w_f32, sl[n].b, w[n] + V);
+      load_weights<T, V>(p.w[kind], p.w_f32, sl[n].a, f);
+      load_weights<T, V>(p.w[kind], p.w_f32, sl[n].b, f + V);
     }
 #pragma unroll
-    for (int i = 0; i < 2 * V; ++i) dw[n][i] = 0.f;
+    for (int k = 0; k < V; ++k) {
+      w[n][k] = pair(f[2 * k], f[2 * k + 1]);
+      dw[n][k] = pair(0.f, 0.f);
+    }
   }
-  const long long units = (long long)p.batch * p.seq * hblocks;
+  const int groups = args.groups[kind], units = p.batch * p.seq * groups;  // (the launcher keeps them below 2^30)
   const float inv_d = 1.f / (float)p.D;
-  for (long long u = (long long)blk * kWarps + warp; u < units; u += (long long)args.nb[kind] * kWarps) {
-    const long long row = u / hblocks;
-    const int hblk = (int)(u - row * hblocks);
-    const int b = (int)(row / p.seq), s = (int)(row - (long long)b * p.seq);
-    const T* xs = reinterpret_cast<const T*>(in.p) + b * in.sb + s * in.ss;
-    const T* gs = reinterpret_cast<const T*>(gr.p) + b * gr.sb + s * gr.ss;
-    T* ds = reinterpret_cast<T*>(const_cast<void*>(o.p)) + b * o.sb + s * o.ss;
-    Pack<T, V> rx[HPT][NSL][2], rg[HPT][NSL][2];
-#pragma unroll
-    for (int h = 0; h < HPT; ++h) {
-      const int head = hblk * args.hb + h * per + sub;
-#pragma unroll
-      for (int n = 0; n < NSL; ++n)
-        if (head < in.heads && sl[n].on) {
-          rx[h][n][0].load(xs + head * in.sh + sl[n].a);
-          rx[h][n][1].load(xs + head * in.sh + sl[n].b);
-          rg[h][n][0].load(gs + head * gr.sh + sl[n].a);
-          rg[h][n][1].load(gs + head * gr.sh + sl[n].b);
-        }
-    }
+  const long long xstep = per * in.sh, gstep = per * gr.sh, dstep = per * o.sh;
+  for (int u = blk * kWarps + warp; u < units; u += args.nb[kind] * kWarps) {
+    const int row = groups == 1 ? u : batch_of(u, groups, args.groups_inv[kind]), group = u - row * groups;
+    const int b = batch_of(row, p.seq, args.seq_inv), s = row - b * p.seq;
     const int pos = p.pos[b * p.pos_sb + s * p.pos_ss];
     const bool in_table = pos >= 0 && pos < p.max_pos;
-    float c[NSL][V], sn[NSL][V];
+    Turn<V, INTER> turn[NSL];
 #pragma unroll
-    for (int n = 0; n < NSL; ++n) {
-      load_angles<V>(p.cos_t, p.sin_t, in_table ? pos : 0, sl[n].j, half, sl[n].on, c[n], sn[n]);
+    for (int n = 0; n < NSL; ++n)
+      turn[n].load(p.cos_t, p.sin_t, in_table ? pos : 0, sl[n].j, half, sl[n].on, -1.f, nullptr);
+    for (int hblk = group * args.inner; hblk < min(hblocks, (group + 1) * args.inner); ++hblk) {
+      const int head0 = hblk * args.hb + sub;
+      const T* xs = reinterpret_cast<const T*>(in.p) + b * in.sb + s * in.ss + head0 * in.sh;
+      const T* gs = reinterpret_cast<const T*>(gr.p) + b * gr.sb + s * gr.ss + head0 * gr.sh;
+      T* ds = reinterpret_cast<T*>(const_cast<void*>(o.p)) + b * o.sb + s * o.ss + head0 * o.sh;
+      if (!in_table) {  // a padded row: zeros, and no share of dw
 #pragma unroll
-      for (int i = 0; i < V; ++i) sn[n][i] = -sn[n][i];
-    }
+        for (int h = 0; h < HPT; ++h, ds += dstep)
 #pragma unroll
-    for (int h = 0; h < HPT; ++h) {
-      const int head = hblk * args.hb + h * per + sub;
-      const bool live = head < in.heads;
-      float x[NSL][2 * V], g[NSL][2 * V], ss = 0.f, sg = 0.f;
+          for (int n = 0; n < NSL; ++n)
+            if (head0 + h * per < in.heads && sl[n].on) store_zeros<T, V>(ds + sl[n].a, ds + sl[n].b);
+        continue;
+      }
+      Pack<T, V> rx[HPT][NSL][2], rg[HPT][NSL][2];
 #pragma unroll
-      for (int n = 0; n < NSL; ++n)
-        if (live && sl[n].on) {
-          rx[h][n][0].to_float(x[n]);
-          rx[h][n][1].to_float(x[n] + V);
-          rg[h][n][0].to_float(g[n]);
-          rg[h][n][1].to_float(g[n] + V);
-          rotate<V>(g[n], c[n], sn[n], sl[n].j, half, p.interleaved);
+      for (int h = 0; h < HPT; ++h, xs += xstep, gs += gstep)
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) {
-            ss += x[n][i] * x[n][i];
-            sg += x[n][i] * g[n][i] * w[n][i];
+        for (int n = 0; n < NSL; ++n)
+          if (head0 + h * per < in.heads && sl[n].on) {
+            rx[h][n][0].load(xs + sl[n].a);
+            rx[h][n][1].load(xs + sl[n].b);
+            rg[h][n][0].load(gs + sl[n].a);
+            rg[h][n][1].load(gs + sl[n].b);
           }
-        }
-      ss = group_sum(ss, gl);
-      sg = group_sum(sg, gl);
-      const float rstd = rsqrtf(ss * inv_d + p.eps);
-      const float m = sg * rstd * inv_d;  // mean(w g h)
 #pragma unroll
-      for (int n = 0; n < NSL; ++n)
-        if (live && sl[n].on) {
-          float d[2 * V];
+      for (int h = 0; h < HPT; ++h, ds += dstep) {
+        const bool live = head0 + h * per < in.heads;
+        uint64_t x[NSL][V], g[NSL][V], ss = pair(0.f, 0.f), sg = pair(0.f, 0.f);
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) {
-            const float hx = x[n][i] * rstd;
-            d[i] = in_table ? rstd * (w[n][i] * g[n][i] - hx * m) : 0.f;
-            if (in_table) dw[n][i] += g[n][i] * hx;
+        for (int n = 0; n < NSL; ++n)
+          if (live && sl[n].on) {
+            to_pairs(rx[h][n][0], rx[h][n][1], x[n]);
+            to_pairs(rg[h][n][0], rg[h][n][1], g[n]);
+            turn[n].apply(g[n], sl[n].j, half, false);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+              ss = fma2(x[n][k], x[n][k], ss);
+              sg = fma2(x[n][k], mul2(g[n][k], w[n][k]), sg);
+            }
           }
-          Pack<T, V> ov;
-          ov.from_float(d);
-          ov.store(ds + head * o.sh + sl[n].a);
-          ov.from_float(d + V);
-          ov.store(ds + head * o.sh + sl[n].b);
-        }
+        const float sx = group_sum(sum2(ss), gl), sxg = group_sum(sum2(sg), gl);
+        const float r = rsqrtf(sx * inv_d + p.eps);
+        const float m = -(r * sxg * inv_d) * r * r;  // -rstd^2 mean(w g h): dx = rstd w g + m x
+        const uint64_t r2 = pair(r, r), m2 = pair(m, m);
+#pragma unroll
+        for (int n = 0; n < NSL; ++n)
+          if (live && sl[n].on) {
+            uint64_t d[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+              const uint64_t gr2 = mul2(g[n][k], r2);  // rstd g
+              d[k] = fma2(x[n][k], m2, mul2(gr2, w[n][k]));
+              dw[n][k] = fma2(gr2, x[n][k], dw[n][k]);
+            }
+            store_pairs<T, V>(d, ds + sl[n].a, ds + sl[n].b);
+          }
+      }
     }
   }
 #pragma unroll
   for (int n = 0; n < NSL; ++n)
 #pragma unroll
-    for (int i = 0; i < 2 * V; ++i) {
-      float v = dw[n][i];
-      for (int k = gl; k < 32; k <<= 1) v += __shfl_xor_sync(0xffffffffu, v, k);
-      if (sub == 0 && sl[n].on) sdw[warp * p.D + (i < V ? sl[n].a + i : sl[n].b + i - V)] = v;
+    for (int k = 0; k < V; ++k) {
+      float v[2];
+      unpair(dw[n][k], v[0], v[1]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        for (int q = gl; q < 32; q <<= 1) v[h] += __shfl_xor_sync(0xffffffffu, v[h], q);
+        const int e = 2 * k + h;
+        if (sub == 0 && sl[n].on) sdw[warp * p.D + (e < V ? sl[n].a + e : sl[n].b + e - V)] = v[h];
+      }
     }
   __syncthreads();
   for (int d = threadIdx.x; d < p.D; d += kThreads) {
@@ -439,6 +541,9 @@ int vector_of(const RotaryParams& p, int esize, bool backward) {
   };
   for (; v > 1; v /= 2) {
     bool ok = p.D % (2 * v) == 0 && (p.interleaved || (p.rot / 2) % v == 0);
+    const size_t wb = p.w_f32 ? std::min(16, 4 * v) : (size_t)esize * v;
+    for (const void* w : p.w) ok = ok && reinterpret_cast<uintptr_t>(w) % wb == 0;
+    ok = ok && reinterpret_cast<uintptr_t>(p.bias) % ((size_t)esize * v) == 0;
     for (int i = 0; i < 3; ++i) ok = ok && fits(p.in[i], v);
     for (int i = 0; i < 2; ++i) {
       if (p.append && i == 1) continue;  // k and v go to the caches, whose rows are D apart (the binding checks 16-byte bases)
@@ -460,18 +565,42 @@ bool valid(const RotaryParams& p) {
          p.seq > 0 && p.max_pos > 0;
 }
 
-template <typename T, int V, int NSL, int HPT>
+int log2_of(int x) {
+  int r = 0;
+  while ((1 << r) < x) ++r;
+  return r;
+}
+// rows < 2^31 / seq * ... : the high word is exact while rows * seq < 2^32
+uint32_t inverse_of(long long rows, int seq) {
+  return seq > 1 && rows * seq < (1ll << 32) ? (uint32_t)(((1ull << 32) + seq - 1) / seq) : 0u;
+}
+
+template <typename T, int V, int NSL, int HPT, int MODE, bool INTER>
 cudaError_t launch_fwd(const RotaryParams& p, cudaStream_t s) {
   RotaryArgs a;
   a.p = p;
   a.gl = lanes_of(p.D / (2 * V));
+  a.gl_shift = log2_of(a.gl);
   a.hb = 32 / a.gl * HPT;
+  const long long rows = (long long)p.batch * p.seq;
   long long hblocks = 0;
   for (int i = 0; i < 3; ++i) hblocks += a.blocks[i] = (p.in[i].heads + a.hb - 1) / a.hb;
-  const long long units = hblocks * p.batch * p.seq, grid = (units + kWarps - 1) / kWarps;
-  if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
-  if (grid == 0) return cudaSuccess;
-  return launch_k(k_rotary<T, V, NSL, HPT>, dim3((unsigned)grid), dim3(kThreads), 0, s, a);
+  a.wh_shift = hblocks >= 4 ? 2 : hblocks >= 2 ? 1 : 0;
+  const int wh = 1 << a.wh_shift;
+  a.seq_inv = inverse_of(rows, p.seq);
+  const int per = kWarps / wh;
+  if (rows >= 0x7fffffffll - kWarps || hblocks > 65535ll * wh) return cudaErrorInvalidValue;
+  if (hblocks == 0) return cudaSuccess;
+  return launch_k(k_rotary<T, V, NSL, HPT, MODE, INTER>, dim3((unsigned)((rows + per - 1) / per), (unsigned)((hblocks + wh - 1) / wh)),
+                  dim3(kThreads), 0, s, a);
+}
+
+template <typename T, int HPT, bool INTER>
+cudaError_t wide_fwd(const RotaryParams& p, cudaStream_t s) {
+  constexpr int VM = 16 / (int)sizeof(T);
+  if (p.append)
+    return p.w[0] ? launch_fwd<T, VM, 1, HPT, kAppendNorm, INTER>(p, s) : launch_fwd<T, VM, 1, HPT, kAppend, INTER>(p, s);
+  return p.w[0] ? launch_fwd<T, VM, 1, HPT, kNorm, INTER>(p, s) : launch_fwd<T, VM, 1, HPT, kPlain, INTER>(p, s);
 }
 
 template <typename T>
@@ -481,11 +610,17 @@ cudaError_t forward_t(const RotaryParams& p, cudaStream_t s) {
   if (v == VM && p.D / (2 * VM) <= 32) {
     const long long heads = (long long)p.batch * p.seq * (p.in[0].heads + p.in[1].heads + p.in[2].heads);
     const int per = 32 / lanes_of(p.D / (2 * VM));
-    return heads >= 148ll * 64 * per ? launch_fwd<T, VM, 1, 4>(p, s) : launch_fwd<T, VM, 1, 1>(p, s);
+    const bool many = heads >= 148ll * 64 * per;
+    if (p.interleaved) return many ? wide_fwd<T, 4, true>(p, s) : wide_fwd<T, 1, true>(p, s);
+    return many ? wide_fwd<T, 4, false>(p, s) : wide_fwd<T, 1, false>(p, s);
   }
-  if (v >= 4) return launch_fwd<T, 4, 2, 1>(p, s);
-  if (v == 2) return launch_fwd<T, 2, 4, 1>(p, s);
-  return launch_fwd<T, 1, 8, 1>(p, s);
+  auto narrow = [&](auto inter) {
+    constexpr bool I = decltype(inter)::value;
+    if (v >= 4) return launch_fwd<T, 4, 2, 1, kAnything, I>(p, s);
+    if (v == 2) return launch_fwd<T, 2, 4, 1, kAnything, I>(p, s);
+    return launch_fwd<T, 1, 8, 1, kAnything, I>(p, s);
+  };
+  return p.interleaved ? narrow(std::true_type{}) : narrow(std::false_type{});
 }
 
 // blocks of the backward: enough to fill the GPU, shared between q and k by their heads
@@ -498,7 +633,7 @@ void bwd_blocks(const RotaryParams& p, int nb[2]) {
   }
 }
 
-template <typename T, int V, int NSL, int HPT>
+template <typename T, int V, int NSL, int HPT, bool INTER>
 cudaError_t launch_bwd(const RotaryParams& p, float* ws, cudaStream_t s) {
   RotaryBwdArgs a;
   a.p = p;
@@ -506,8 +641,18 @@ cudaError_t launch_bwd(const RotaryParams& p, float* ws, cudaStream_t s) {
   a.hb = 32 / a.gl * HPT;
   a.ws = ws;
   bwd_blocks(p, a.nb);
-  for (int i = 0; i < 2; ++i) a.blocks[i] = (p.in[i].heads + a.hb - 1) / a.hb;
-  return launch_k(k_rotary_norm_bwd<T, V, NSL, HPT>, dim3(a.nb[0] + a.nb[1]), dim3(kThreads),
+  const long long rows = (long long)p.batch * p.seq;
+  a.gl_shift = log2_of(a.gl);
+  a.seq_inv = inverse_of(rows, p.seq);
+  // rows alone fill the GPU: a warp keeps a row's angles for four head blocks, else for one
+  a.inner = rows >= 148 * 24 ? 4 : 1;
+  for (int i = 0; i < 2; ++i) {
+    a.blocks[i] = (p.in[i].heads + a.hb - 1) / a.hb;
+    a.groups[i] = (a.blocks[i] + a.inner - 1) / a.inner;
+    a.groups_inv[i] = inverse_of(rows * a.groups[i], a.groups[i]);
+    if (rows * a.groups[i] >= (1ll << 30)) return cudaErrorInvalidValue;
+  }
+  return launch_k(k_rotary_norm_bwd<T, V, NSL, HPT, INTER>, dim3(a.nb[0] + a.nb[1]), dim3(kThreads),
                   (size_t)kWarps * p.D * sizeof(float), s, a);
 }
 
@@ -515,10 +660,14 @@ template <typename T>
 cudaError_t backward_t(const RotaryParams& p, float* ws, cudaStream_t s) {
   constexpr int VM = 16 / (int)sizeof(T);
   const int v = vector_of(p, sizeof(T), true);
-  if (v == VM && p.D / (2 * VM) <= 32) return launch_bwd<T, VM, 1, 2>(p, ws, s);
-  if (v >= 4) return launch_bwd<T, 4, 2, 1>(p, ws, s);
-  if (v == 2) return launch_bwd<T, 2, 4, 1>(p, ws, s);
-  return launch_bwd<T, 1, 8, 1>(p, ws, s);
+  auto go = [&](auto inter) {
+    constexpr bool I = decltype(inter)::value;
+    if (v == VM && p.D / (2 * VM) <= 32) return launch_bwd<T, VM, 1, 2, I>(p, ws, s);
+    if (v >= 4) return launch_bwd<T, 4, 2, 1, I>(p, ws, s);
+    if (v == 2) return launch_bwd<T, 2, 4, 1, I>(p, ws, s);
+    return launch_bwd<T, 1, 8, 1, I>(p, ws, s);
+  };
+  return p.interleaved ? go(std::true_type{}) : go(std::false_type{});
 }
 
 }  // namespace

@@ -156,6 +156,27 @@ Tensor py_rotary(Tensor x, Tensor positions, Tensor cos_t, Tensor sin_t, bool in
   return y;
 }
 
+// y = R x; the gradient of a rotation is the rotation back (itself differentiable)
+struct RotaryFn : public torch::autograd::Function<RotaryFn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor x, Tensor positions, Tensor cos_t, Tensor sin_t,
+                        bool interleaved, bool inverse) {
+    ctx->save_for_backward({positions, cos_t, sin_t});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    return py_rotary(x, positions, cos_t, sin_t, interleaved, inverse, c10::nullopt);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dy) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor dx = RotaryFn::apply(dy[0], s[0], s[1], s[2], ctx->saved_data["interleaved"].toBool(),
+                                      !ctx->saved_data["inverse"].toBool());
+    return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor py_rotary_autograd(Tensor x, Tensor positions, Tensor cos_t, Tensor sin_t, bool interleaved, bool inverse) {
+  return RotaryFn::apply(x, positions, cos_t, sin_t, interleaved, inverse);
+}
+
 void weights_ok(const Tensor& wq, const Tensor& wk, const Tensor& x, cob::RotaryParams& p) {
   for (const auto* w : {&wq, &wk}) {
     on_device(*w, "norm weight", x);
@@ -248,6 +269,31 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> py_qk_norm_rotary_backward(Tensor dq,
   Tensor ws = torch::empty({cob::rotary_backward_blocks(p), q.size(-1)}, wq.options().dtype(torch::kFloat).requires_grad(false));
   ok(cob::rotary_norm_backward(p, ws.data_ptr<float>(), gwq.data_ptr(), gwk.data_ptr(), cur()), "qk_norm_rotary backward");
   return {gq, gk, gwq, gwk};
+}
+
+struct QkNormRotaryFn : public torch::autograd::Function<QkNormRotaryFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, Tensor q, Tensor k, Tensor wq,
+                                                Tensor wk, Tensor positions, Tensor cos_t, Tensor sin_t, double eps,
+                                                bool interleaved) {
+    ctx->save_for_backward({q, k, wq, wk, positions, cos_t, sin_t});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    auto y = py_qk_norm_rotary(q, k, wq, wk, positions, cos_t, sin_t, eps, interleaved);
+    return {std::get<0>(y), std::get<1>(y)};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dy) {
+    COB_CHECK(!torch::GradMode::is_enabled(), "qk_norm_rotary: gradients of its gradients are not formed");
+    const auto s = ctx->get_saved_variables();
+    auto g = py_qk_norm_rotary_backward(dy[0], dy[1], s[0], s[1], s[2], s[3], s[4], s[5], s[6],
+                                        ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool());
+    return {std::get<0>(g), std::get<1>(g), std::get<2>(g), std::get<3>(g), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> py_qk_norm_rotary_autograd(Tensor q, Tensor k, Tensor wq, Tensor wk, Tensor positions,
+                                                      Tensor cos_t, Tensor sin_t, double eps, bool interleaved) {
+  auto y = QkNormRotaryFn::apply(q, k, wq, wk, positions, cos_t, sin_t, eps, interleaved);
+  return {y[0], y[1]};
 }
 
 // caches [num_blocks, nkv, 16, D] and block tables [batch, max_blocks]
@@ -523,7 +569,9 @@ Tensor py_penalize_logits(Tensor logits, OptTensor tokens, OptTensor lens, OptTe
 
 void register_serve(pybind11::module& m) {
   m.def("rotary", &py_rotary);
+  m.def("rotary_autograd", &py_rotary_autograd);
   m.def("qk_norm_rotary", &py_qk_norm_rotary);
+  m.def("qk_norm_rotary_autograd", &py_qk_norm_rotary_autograd);
   m.def("qk_norm_rotary_backward", &py_qk_norm_rotary_backward);
   m.def("qk_norm_rotary_append", &py_qk_norm_rotary_append);
   m.def("tree_attention", &py_tree_attention);

@@ -9,7 +9,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .._ext import native
 
@@ -66,19 +65,6 @@ def rotary_tables(max_pos: int, rotary_dim: int, theta: float = 10000.0, scaling
     return (ang.cos() * mul).float().to(device), (ang.sin() * mul).float().to(device)
 
 
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, positions, cos, sin, interleaved, inverse):
-        ctx.save_for_backward(positions, cos, sin)
-        ctx.layout = interleaved, inverse
-        return native().rotary(x, positions, cos, sin, interleaved, inverse, None)
-
-    @staticmethod
-    def backward(ctx, dy):
-        interleaved, inverse = ctx.layout  # the gradient of a rotation is the rotation back
-        return _Rotary.apply(dy, *ctx.saved_tensors, interleaved, not inverse), None, None, None, None, None
-
-
 def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, interleaved: bool = False,
            inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotate x [tokens, heads, D] or [batch, seq, heads, D] (fp32, fp16, bf16; any strides) by its positions
@@ -87,25 +73,10 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: tor
     Differentiable in x. ``inverse`` rotates back. ``out`` may be x (in place, no gradient) or other memory. A row whose
     position lies outside the tables becomes zeros (and has a zero gradient): padded rows carry position -1."""
     if out is None and x.requires_grad and torch.is_grad_enabled():
-        return _Rotary.apply(x, positions, cos, sin, bool(interleaved), bool(inverse))
+        return native().rotary_autograd(x, positions, cos, sin, bool(interleaved), bool(inverse))
     if out is not None and torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
         raise RuntimeError("rotary with out= forms no gradient: call it without out, or under torch.no_grad()")
     return native().rotary(x, positions, cos, sin, bool(interleaved), bool(inverse), out)
-
-
-class _QkNormRotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved):
-        ctx.save_for_backward(q, k, q_weight, k_weight, positions, cos, sin)
-        ctx.eps, ctx.interleaved = eps, interleaved
-        return native().qk_norm_rotary(q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk):
-        q, k, wq, wk, positions, cos, sin = ctx.saved_tensors
-        grads = native().qk_norm_rotary_backward(dq, dk, q, k, wq, wk, positions, cos, sin, ctx.eps, ctx.interleaved)
-        return (*grads, None, None, None, None, None)
 
 
 def qk_norm_rotary(q, k, q_weight, k_weight, positions, cos, sin, eps: float = 1e-6, *, interleaved: bool = False):
@@ -117,7 +88,7 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, cos, sin, eps: float = 1
     capture it in a CUDA graph)."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or
                                     k_weight.requires_grad):
-        return _QkNormRotary.apply(q, k, q_weight, k_weight, positions, cos, sin, float(eps), bool(interleaved))
+        return native().qk_norm_rotary_autograd(q, k, q_weight, k_weight, positions, cos, sin, float(eps), bool(interleaved))
     return native().qk_norm_rotary(q, k, q_weight, k_weight, positions, cos, sin, float(eps), bool(interleaved))
 
 

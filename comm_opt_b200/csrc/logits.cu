@@ -41,15 +41,18 @@ struct RowScalars {
   }
 };
 
-template <typename T>
+// `chunk` ids of one row; MAXV: 16-byte vectors of them per thread
+template <typename T, int MAXV>
 __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ LogitsParams p, int chunk, int counts,
                                                        int biases) {
   using V = Vec<T>;
+  constexpr int N = V::N;
   extern __shared__ __align__(16) uint32_t sm[];
-  __shared__ float sval[32];
-  __shared__ unsigned long long skey[kThreads / 32];
+  __shared__ int s_id[kThreads];
+  __shared__ float s_val[kThreads];
+  __shared__ unsigned long long s_key[kThreads / 32];
   pdl_wait_then_trigger();
-  const int row = blockIdx.x;
+  const int row = blockIdx.x, tid = threadIdx.x;
   const T* in = reinterpret_cast<const T*>(p.logits) + row * p.ld_in;
   T* out = reinterpret_cast<T*>(p.out) + row * p.ld_out;
   // ids up to the row's first 16-byte boundary belong to the first chunk; every chunk then starts on one
@@ -60,49 +63,49 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
   const int lo = blockIdx.y == 0 ? 0 : v0;  // first id of this CTA
   const int n = v1 - lo;
   if (n <= 0) return;
-  const int slots = chunk + V::N;
-  uint32_t* cnt = sm;
-  float* bsum = reinterpret_cast<float*>(sm + (counts ? slots : 0));
-  const int words = (counts ? slots : 0) + (biases ? slots : 0);
-  for (int i = threadIdx.x; i < words; i += kThreads) sm[i] = 0u;
-  __syncthreads();
-  const int g0 = p.vocab_offset + lo;  // global id of slot 0
+  const int nv = (v1 - v0) / N;  // whole vectors
+  const int g0 = p.vocab_offset + lo;  // first global id
+  // Everything this CTA reads first is requested at once: the chunk, its mask words, the row's scalars, a tile of the
+  // biases and a tile of the history (whose length is only applied afterwards), one memory latency for all.
+  uint4 raw[MAXV];
+  const uint32_t* mask = p.allowed ? p.allowed + row * p.ld_mask : nullptr;
+#pragma unroll
+  for (int i = 0; i < MAXV; ++i) {
+    const int e = tid + i * kThreads;
+    if (e < nv) {
+      raw[i] = *reinterpret_cast<const uint4*>(in + v0 + e * N);
+    }
+  }
+  // bit words of the chunk's ids v0 + 32 w ..: allowed, and touched by the history or a bias
+  constexpr int kWords = MAXV * N * kThreads / 32, kPer = (kWords + kThreads - 1) / kThreads;
+  __shared__ uint32_t s_mask[kWords], s_mark[kWords + 1];  // (one more for the ids before v0)
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int w = tid + i * kThreads, g = p.vocab_offset + v0 + 32 * w;
+    if (w < kWords) {
+      s_mark[w] = 0;
+      if (mask && 32 * w < v1 - v0) {
+        const uint32_t a = __ldg(mask + (g >> 5));
+        const uint32_t b = (g & 31) && ((g >> 5) + 1) * 32 < p.vocab_offset + p.vocab ? __ldg(mask + (g >> 5) + 1) : 0u;
+        s_mask[w] = __funnelshift_r(a, b, g & 31);
+      }
+    }
+  }
+  constexpr int kTile = 4;
+  const int32_t* tok = p.tokens + row * p.ld_tokens;
+  int t[kTile];
+  int len = 0, plen = 0;
   if (counts) {
-    const int32_t* tok = p.tokens + row * p.ld_tokens;
-    const int len = p.lens ? min(max(p.lens[row], 0), p.history) : p.history;
-    const int plen = p.prompt_lens ? p.prompt_lens[row] : 0;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < len; i += kThreads) {
-      const unsigned id = (unsigned)(tok[i] - g0);
-      if (tok[i] >= g0 && id < (unsigned)n) {
-        if (i < plen)
-          atomicOr(cnt + id, kInPrompt);
-        else
-          atomicAdd(cnt + id, 1u);
-      }
-    }
+    len = p.lens ? min(max(p.lens[row], 0), p.history) : p.history;
+    plen = p.prompt_lens ? p.prompt_lens[row] : 0;
+#pragma unroll
+    for (int k = 0; k < kTile; ++k) t[k] = tid + k * kThreads < p.history ? tok[tid + k * kThreads] : -1;
   }
-  if (biases && threadIdx.x < 32) {  // one warp, 32 entries at a time: equal ids add up in their order
-    const int32_t* ids = p.bias_ids + (size_t)row * p.biases;
-    const float* val = p.bias + (size_t)row * p.biases;
-    const int lane = threadIdx.x;
-    for (int i0 = 0; i0 < p.biases; i0 += 32) {
-      const int i = i0 + lane;
-      const int id = i < p.biases ? ids[i] : -1;
-      const bool mine = id >= g0 && (unsigned)(id - g0) < (unsigned)n;
-      if (!__any_sync(0xffffffffu, mine)) continue;
-      sval[lane] = mine ? val[i] : 0.f;
-      const unsigned same = __match_any_sync(0xffffffffu, mine ? id : -1 - lane);
-      __syncwarp();
-      if (mine && (same & ((1u << lane) - 1u)) == 0) {
-        float s = bsum[id - g0];
-        for (unsigned m = same; m; m &= m - 1) s = __fadd_rn(s, sval[__ffs(m) - 1]);
-        bsum[id - g0] = s;
-      }
-      __syncwarp();
-    }
-  }
-  __syncthreads();
+  const int32_t* ids = p.bias_ids + (size_t)row * p.biases;
+  const float* val = p.bias + (size_t)row * p.biases;
+  int bid = -1;
+  float bval = 0.f;
+  if (biases && tid < p.biases) bid = ids[tid], bval = val[tid];
   RowScalars r;
   r.has_rep = p.repetition != nullptr;
   r.has_freq = p.frequency != nullptr;
@@ -110,52 +113,135 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
   r.rep = r.has_rep ? p.repetition[row] : 1.f;
   r.freq = r.has_freq ? p.frequency[row] : 0.f;
   r.pres = r.has_pres ? p.presence[row] : 0.f;
-  const uint32_t* mask = p.allowed ? p.allowed + row * p.ld_mask : nullptr;
-  unsigned long long best = 0ull;
-  auto one = [&](float x, int v) {  // v: id within this shard
-    if (counts) x = r.apply(x, cnt[v - lo]);
-    if (biases) x = __fadd_rn(x, bsum[v - lo]);
-    if (mask) {
-      const int g = p.vocab_offset + v;
-      if (!((__ldg(mask + (g >> 5)) >> (g & 31)) & 1u)) x = -INFINITY;
+  // id v has slot v - v0 + N of the tables (the few ids before v0 sit in the first N), so vectors are aligned there too
+  const int slots = chunk + 2 * N, base = N - v0;
+  uint32_t* cnt = sm;
+  float* bsum = reinterpret_cast<float*>(sm + (counts ? slots : 0));
+  const int words4 = ((counts ? slots : 0) + (biases ? slots : 0)) / 4;
+  for (int i = tid; i < words4; i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
+  const int gs = p.vocab_offset - base;  // global id of slot 0
+  auto mark = [&](int slot) {
+    if (slot >= N) atomicOr(&s_mark[(slot - N) >> 5], 1u << ((slot - N) & 31));
+  };
+  // biases in tiles of one entry per thread; one warp adds them up 32 at a time, equal ids in their order
+  for (int i0 = 0;;) {
+    const bool mine = bid >= g0 && bid - g0 < n;
+    s_id[tid] = mine ? bid - gs : -1;
+    s_val[tid] = bval;
+    const int here = biases ? min(kThreads, p.biases - i0) : 0;
+    i0 += kThreads;
+    const bool more = biases && i0 < p.biases;
+    if (more) {
+      bid = i0 + tid < p.biases ? ids[i0 + tid] : -1;
+      bval = i0 + tid < p.biases ? val[i0 + tid] : 0.f;
     }
-    return x;
-  };
-  auto single = [&](int v) {
-    const T o = from_f<T>(one(to_f(in[v]), v));
-    out[v] = o;
-    if (p.keys) best = max(best, greedy_key(to_f(o), (uint32_t)(p.vocab_offset + v)));
-  };
-  const int nv = (v1 - v0) / V::N;  // whole vectors
-  const bool vec_store = ((reinterpret_cast<uintptr_t>(out + v0)) & 15) == 0;
-  for (int i = threadIdx.x; i < nv; i += kThreads) {
-    const int v = v0 + i * V::N;
-    float f[V::N];
-    V::to_float(*reinterpret_cast<const uint4*>(in + v), f);
+    __syncthreads();  // (the first also completes the tables' zeros)
+    if (tid < 32)
+      for (int t0 = 0; t0 < here; t0 += 32) {
+        const int at = s_id[t0 + tid];
+        if (!__any_sync(0xffffffffu, at >= 0)) continue;
+        const unsigned same = __match_any_sync(0xffffffffu, at >= 0 ? at : -1 - tid);
+        if (at >= 0 && (same & ((1u << tid) - 1u)) == 0) {
+          float s = bsum[at];
+          for (unsigned m = same; m; m &= m - 1) s = __fadd_rn(s, s_val[t0 + __ffs(m) - 1]);
+          bsum[at] = s;
+          mark(at);
+        }
+        __syncwarp();
+      }
+    if (!more) break;
+    __syncthreads();
+  }
+  if (counts) {
+    for (int i0 = tid; i0 < len;) {
+      int ahead[kTile];  // the next tile is on its way while this one is counted
 #pragma unroll
-    for (int j = 0; j < V::N; ++j) f[j] = one(f[j], v + j);
+      for (int k = 0; k < kTile; ++k) {
+        const int i = i0 + (kTile + k) * kThreads;
+        ahead[k] = i < len ? tok[i] : -1;
+      }
+#pragma unroll
+      for (int k = 0; k < kTile; ++k) {
+        const int i = i0 + k * kThreads;
+        if (i < len && t[k] >= g0 && t[k] - g0 < n) {
+          mark(t[k] - gs);
+          if (i < plen)
+            atomicOr(cnt + (t[k] - gs), kInPrompt);
+          else
+            atomicAdd(cnt + (t[k] - gs), 1u);
+        }
+      }
+      i0 += kTile * kThreads;
+#pragma unroll
+      for (int k = 0; k < kTile; ++k) t[k] = ahead[k];
+    }
+  }
+  unsigned long long best = 0ull;
+  __syncthreads();
+  auto single = [&](int v) {
+    float x = to_f(in[v]);
+    if (counts) x = r.apply(x, cnt[v + base]);
+    if (biases) x = __fadd_rn(x, bsum[v + base]);
+    const int g = p.vocab_offset + v;
+    if (mask && !((__ldg(mask + (g >> 5)) >> (g & 31)) & 1u)) x = -INFINITY;
+    const T o = from_f<T>(x);
+    out[v] = o;
+    if (p.keys) best = max(best, greedy_key(to_f(o), (uint32_t)g));
+  };
+  const bool vec_store = ((reinterpret_cast<uintptr_t>(out + v0)) & 15) == 0;
+#pragma unroll
+  for (int i = 0; i < MAXV; ++i) {
+    const int e = tid + i * kThreads;
+    if (e >= nv) break;
+    const int v = v0 + e * N, slot = N + e * N, g = p.vocab_offset + v;
+    float f[N];
+    V::to_float(raw[i], f);
+    const int word = e * N >> 5, bit = e * N & 31;  // a vector's bits lie in one word
+    if ((s_mark[word] >> bit) & ((1u << N) - 1u)) {
+      if (counts) {
+        uint32_t c[N];
+#pragma unroll
+        for (int j = 0; j < N; j += 4) *reinterpret_cast<uint4*>(c + j) = *reinterpret_cast<const uint4*>(cnt + slot + j);
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = r.apply(f[j], c[j]);
+      }
+      if (biases) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(bsum + slot + j);
+          f[j] = __fadd_rn(f[j], b.x), f[j + 1] = __fadd_rn(f[j + 1], b.y);
+          f[j + 2] = __fadd_rn(f[j + 2], b.z), f[j + 3] = __fadd_rn(f[j + 3], b.w);
+        }
+      }
+    }
+    if (mask) {
+      const uint32_t bits = s_mask[word] >> bit;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (!((bits >> j) & 1u)) f[j] = -INFINITY;
+    }
     const uint4 o = V::from_float(f);
     if (vec_store) {
       *reinterpret_cast<uint4*>(out + v) = o;
     } else {
 #pragma unroll
-      for (int j = 0; j < V::N; ++j) out[v + j] = from_f<T>(f[j]);
+      for (int j = 0; j < N; ++j) out[v + j] = from_f<T>(f[j]);
     }
     if (p.keys) {
       V::to_float(o, f);
 #pragma unroll
-      for (int j = 0; j < V::N; ++j) best = max(best, greedy_key(f[j], (uint32_t)(p.vocab_offset + v + j)));
+      for (int j = 0; j < N; ++j) best = max(best, greedy_key(f[j], (uint32_t)(g + j)));
     }
   }
-  for (int v = lo + threadIdx.x; v < v0; v += kThreads) single(v);
-  for (int v = v0 + nv * V::N + threadIdx.x; v < v1; v += kThreads) single(v);
+  for (int v = lo + tid; v < v0; v += kThreads) single(v);
+  for (int v = v0 + nv * N + tid; v < v1; v += kThreads) single(v);
   if (!p.keys) return;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if ((threadIdx.x & 31) == 0) skey[threadIdx.x >> 5] = best;
+  if ((tid & 31) == 0) s_key[tid >> 5] = best;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kThreads / 32; ++w) best = max(best, skey[w]);
+  if (tid == 0) {
+    for (int w = 1; w < kThreads / 32; ++w) best = max(best, s_key[w]);
     atomicMax(p.keys + row, best);
   }
 }
@@ -164,12 +250,13 @@ template <typename T>
 cudaError_t launch(const LogitsParams& p, cudaStream_t s) {
   const int counts = p.tokens != nullptr && p.history > 0 && (p.repetition || p.frequency || p.presence);
   const int biases = p.bias != nullptr && p.biases > 0;
-  int chunk = 4096;
+  constexpr int N = Vec<T>::N, kChunk = 4096;
+  int chunk = kChunk;
   while (chunk > 1024 && (long long)p.rows * ((p.vocab + chunk - 1) / chunk) < 148 * 2) chunk /= 2;
-  const size_t smem = (size_t)(counts + biases) * (chunk + Vec<T>::N) * 4;
-  // the leading ids (fewer than a vector) shift the chunks by at most one vector
+  const size_t smem = (size_t)(counts + biases) * (chunk + 2 * N) * 4;
+  // the leading ids (fewer than a vector) shift the chunks by less than one vector
   const dim3 grid(p.rows, (p.vocab + chunk - 1) / chunk);
-  return launch_k(k_penalize<T>, grid, dim3(kThreads), smem, s, p, chunk, counts, biases);
+  return launch_k(k_penalize<T, kChunk / N / kThreads>, grid, dim3(kThreads), smem, s, p, chunk, counts, biases);
 }
 
 }  // namespace

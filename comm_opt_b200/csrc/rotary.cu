@@ -24,6 +24,9 @@ namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kPage = 16;  // tokens per cache page
+// heads that a lane takes per step where there are many rows (measured: 3 without the norm's registers, 166.7 us for the
+// long prompt against 177 with 2; 2 with them, 47.0 us for the padded prompts against 50.7 with 3)
+constexpr int kSteps = 3, kStepsNorm = 2;
 
 // two 16-bit components of a word
 template <typename T>
@@ -178,12 +181,12 @@ template <int V, bool INTER>
 struct Turn {
   static constexpr bool kWithin = INTER || V == 1;
   uint64_t c[V], s[V];
-  __device__ __forceinline__ void load(const float* ct, const float* st, size_t row, int j, int half, bool on, float sign,
+  __device__ __forceinline__ void load(const float* ct, const float* st, size_t row, int j, int half, float sign,
                                        const float* w) {
     float cv[V], sv[V];
     ct += row * half + j;
     st += row * half + j;
-    if (on && V % 4 == 0 && half % 4 == 0 && j + V <= half) {
+    if (V % 4 == 0 && half % 4 == 0 && j + V <= half) {
 #pragma unroll
       for (int i = 0; i + 3 < V; i += 4) {
         const float4 a = __ldg(reinterpret_cast<const float4*>(ct + i)), b = __ldg(reinterpret_cast<const float4*>(st + i));
@@ -193,7 +196,7 @@ struct Turn {
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const bool turns = on && j + i < half;
+        const bool turns = j + i < half;
         cv[i] = turns ? __ldg(ct + i) : 1.f;
         sv[i] = turns ? __ldg(st + i) : 0.f;
       }
@@ -243,8 +246,19 @@ struct Turn {
 };
 
 __device__ __forceinline__ float group_sum(float v, int gl) {
-  for (int o = gl >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < gl) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+// a parameter array's element by value (indexed parameters would be read from constant memory at every use)
+template <typename A>
+__device__ __forceinline__ A pick(const A (&a)[3], int i) {
+  return i == 0 ? a[0] : i == 1 ? a[1] : a[2];
+}
+template <typename A>
+__device__ __forceinline__ A pick(const A (&a)[2], int i) {
+  return i == 0 ? a[0] : a[1];
 }
 
 // What a kernel is compiled for: kAnything decides at run time (the narrow-vector forms)
@@ -253,27 +267,29 @@ enum Mode : int { kPlain = 0, kNorm = 1, kAppend = 2, kAppendNorm = 3, kAnything
 struct RotaryArgs {
   RotaryParams p;
   int gl, gl_shift;  // lanes per head
-  int hb;            // heads per warp
-  int blocks[3];     // head blocks of q, k, v per row
-  int wh_shift;      // log2 of the warps of a block side by side on one row's head blocks (they share its angles in L1)
+  int hb;            // heads per step of a warp
+  int blocks[3];     // head blocks (steps) of q, k, v per row
+  int groups[3];     // warps that share them: `inner` steps each
+  int inner;
+  int wh_shift;      // log2 of the warps of a block side by side on one row's groups (they share its angles in L1)
   uint32_t seq_inv;  // ceil(2^32 / seq): row / seq = high word of row * seq_inv; 0: divide
 };
 __device__ __forceinline__ int batch_of(int row, int seq, uint32_t inv) {
   return inv ? (int)__umulhi((uint32_t)row, inv) : row / seq;
 }
 
-// One warp takes `hb` heads of one row: 32 / gl heads side by side, HPT after one another with all their loads
-// in flight; the angles and weights are loaded and combined once for them.
+// One warp takes `inner` steps of one row's q, k or v heads, the angles and weights loaded and combined once for them. A
+// step is 32 / gl heads side by side, HPT after one another; the next step's loads are in flight while one is computed.
 template <typename T, int V, int NSL, int HPT, int MODE, bool INTER>
-__global__ void __launch_bounds__(kThreads, HPT > 1 ? ((MODE & kNorm) ? 4 : 5) : NSL == 1 ? 6 : 1)
+__global__ void __launch_bounds__(kThreads, HPT > 1 ? 4 : NSL == 1 ? 6 : 1)
     k_rotary(const __grid_constant__ RotaryArgs args) {
   const RotaryParams& p = args.p;
   pdl_wait_then_trigger();
   const int warp = threadIdx.x >> 5;
   const int row = (int)blockIdx.x * (kWarps >> args.wh_shift) + (warp >> args.wh_shift);
-  int hblk = ((int)blockIdx.y << args.wh_shift) + (warp & ((1 << args.wh_shift) - 1)), kind = 0;
-  if (row >= p.batch * p.seq || hblk >= args.blocks[0] + args.blocks[1] + args.blocks[2]) return;
-  while (kind < 2 && hblk >= args.blocks[kind]) hblk -= args.blocks[kind++];
+  int group = ((int)blockIdx.y << args.wh_shift) + (warp & ((1 << args.wh_shift) - 1)), kind = 0;
+  if (row >= p.batch * p.seq || group >= args.groups[0] + args.groups[1] + args.groups[2]) return;
+  while (kind < 2 && group >= args.groups[kind]) group -= args.groups[kind++];
   const bool append = MODE == kAnything ? p.append != 0 : MODE >= kAppend;
   const bool norm = kind < 2 && (MODE == kAnything ? p.w[0] != nullptr : (MODE & kNorm) != 0);
   const bool has_bias = (MODE == kAnything || MODE >= kAppend) && p.bias != nullptr;
@@ -284,32 +300,43 @@ __global__ void __launch_bounds__(kThreads, HPT > 1 ? ((MODE & kNorm) ? 4 : 5) :
   const bool in_table = pos >= 0 && pos < p.max_pos;
   const int start = append && kind > 0 ? p.starts[b] : 0;
   if (append && (!in_table || (p.lens && s >= p.lens[b]))) return;
-  const HeadView& in = p.in[kind];
-  const int head0 = hblk * args.hb + sub;  // this lane's first head, then every `per`-th
-  const T* src = reinterpret_cast<const T*>(in.p) + b * in.sb + s * in.ss + head0 * in.sh;
-  const long long src_step = per * in.sh;
+  const HeadView in = pick(p.in, kind);
+  // Lanes without a slot, and heads past the last one in a warp's row of them, work on copies of real ones and only do not
+  // store, so the arithmetic has no branches; whole steps past the last head are left out.
+  int hblk = group * args.inner;
+  const int hend = min(pick(args.blocks, kind), hblk + args.inner);
   Slot<V> sl[NSL];
+#pragma unroll
+  for (int n = 0; n < NSL; ++n) {
+    sl[n] = slot_of<V, INTER>(min(l + n * gl, nslots - 1), nslots, half);
+    sl[n].on = l + n * gl < nslots;
+  }
+  const T* src = reinterpret_cast<const T*>(in.p) + b * in.sb + s * in.ss;
   Pack<T, V> raw[HPT][NSL][2];
+  auto fetch = [&](int hblk, Pack<T, V>(&r)[HPT][NSL][2]) {
 #pragma unroll
-  for (int n = 0; n < NSL; ++n) sl[n] = slot_of<V, INTER>(l + n * gl, nslots, half);
+    for (int h = 0; h < HPT; ++h)
+      if (HPT == 1 || hblk * args.hb + h * per < in.heads) {
+        const T* at = src + min(hblk * args.hb + h * per + sub, in.heads - 1) * in.sh;
 #pragma unroll
-  for (int h = 0; h < HPT; ++h, src += src_step)
-#pragma unroll
-    for (int n = 0; n < NSL; ++n)
-      if (head0 + h * per < in.heads && sl[n].on) {
-        raw[h][n][0].load(src + sl[n].a);
-        raw[h][n][1].load(src + sl[n].b);
+        for (int n = 0; n < NSL; ++n) {
+          r[h][n][0].load(at + sl[n].a);
+          r[h][n][1].load(at + sl[n].b);
+        }
       }
+  };
+  fetch(hblk, raw);
   Turn<V, INTER> turn[NSL];
   if (kind < 2) {
+    const void* wp = pick(p.w, kind);
 #pragma unroll
     for (int n = 0; n < NSL; ++n) {
       float w[2 * V];
-      if (norm && sl[n].on) {
-        load_weights<T, V>(p.w[kind], p.w_f32, sl[n].a, w);
-        load_weights<T, V>(p.w[kind], p.w_f32, sl[n].b, w + V);
+      if (norm) {
+        load_weights<T, V>(wp, p.w_f32, sl[n].a, w);
+        load_weights<T, V>(wp, p.w_f32, sl[n].b, w + V);
       }
-      turn[n].load(p.cos_t, p.sin_t, in_table ? pos : 0, sl[n].j, half, sl[n].on, p.inverse ? -1.f : 1.f, norm ? w : nullptr);
+      turn[n].load(p.cos_t, p.sin_t, in_table ? pos : 0, sl[n].j, half, p.inverse ? -1.f : 1.f, norm ? w : nullptr);
     }
   }
   T* dst;
@@ -323,60 +350,72 @@ __global__ void __launch_bounds__(kThreads, HPT > 1 ? ((MODE & kNorm) ? 4 : 5) :
     dst = cache + ((long long)blk * in.heads * kPage + slot % kPage) * p.D;
     dst_sh = (long long)kPage * p.D;
   } else {
-    const HeadView& o = p.out[kind];
+    const HeadView o = pick(p.out, kind);
     dst = reinterpret_cast<T*>(const_cast<void*>(o.p)) + b * o.sb + s * o.ss;
     dst_sh = o.sh;
   }
-  dst += head0 * dst_sh;
-  const long long dst_step = per * dst_sh;
-  if (!append && !in_table) {  // a padded row
+  const int bias0 = (kind > 0 ? p.in[0].heads : 0) + (kind > 1 ? p.in[1].heads : 0);  // bias order: q, k, v heads
+  const float inv_d = 1.f / (float)p.D;
+  Pack<T, V> ahead[HPT][NSL][2];
+  for (;;) {
+    const bool more = HPT > 1 && hblk + 1 < hend;  // (HPT = 1 is launched with one step a warp)
+    if (more) fetch(hblk + 1, ahead);
 #pragma unroll
-    for (int h = 0; h < HPT; ++h, dst += dst_step)
+  for (int h = 0; h < HPT; ++h) {
+    if (HPT > 1 && hblk * args.hb + h * per >= in.heads) break;
+    const int head = hblk * args.hb + h * per + sub;
+    T* to = dst + head * dst_sh;
+    uint64_t x[NSL][V];
+    if (!append && !in_table) {  // a padded row
 #pragma unroll
       for (int n = 0; n < NSL; ++n)
-        if (head0 + h * per < in.heads && sl[n].on) store_zeros<T, V>(dst + sl[n].a, dst + sl[n].b);
-    return;
-  }
-  // bias order: q, k, v heads
-  const int bias0 = (kind > 0 ? p.in[0].heads : 0) + (kind > 1 ? p.in[1].heads : 0) + head0;
-  const T* bias = reinterpret_cast<const T*>(p.bias) + (size_t)bias0 * p.D;
+        if (head < in.heads && sl[n].on) store_zeros<T, V>(to + sl[n].a, to + sl[n].b);
+      continue;
+    }
 #pragma unroll
-  for (int h = 0; h < HPT; ++h, dst += dst_step, bias += per * p.D) {
-    const bool live = head0 + h * per < in.heads;
-    uint64_t x[NSL][V], ss = pair(0.f, 0.f);
+    for (int n = 0; n < NSL; ++n) to_pairs(raw[h][n][0], raw[h][n][1], x[n]);
+    if (has_bias) {
+      const T* bias = reinterpret_cast<const T*>(p.bias) + (size_t)(bias0 + min(head, in.heads - 1)) * p.D;
 #pragma unroll
-    for (int n = 0; n < NSL; ++n)
-      if (live && sl[n].on) {
-        to_pairs(raw[h][n][0], raw[h][n][1], x[n]);
-        if (has_bias) {
-          Pack<T, V> b0, b1;
-          b0.load(bias + sl[n].a);
-          b1.load(bias + sl[n].b);
-          uint64_t bf[V];
-          to_pairs(b0, b1, bf);
+      for (int n = 0; n < NSL; ++n) {
+        Pack<T, V> b0, b1;
+        b0.load(bias + sl[n].a);
+        b1.load(bias + sl[n].b);
+        uint64_t bf[V];
+        to_pairs(b0, b1, bf);
 #pragma unroll
-          for (int k = 0; k < V; ++k) x[n][k] = add2(x[n][k], bf[k]);
-        }
-        if (norm) {
-#pragma unroll
-          for (int k = 0; k < V; ++k) ss = fma2(x[n][k], x[n][k], ss);
-        }
+        for (int k = 0; k < V; ++k) x[n][k] = add2(x[n][k], bf[k]);
       }
+    }
     uint64_t rstd = 0;
     if (norm) {
-      const float r = rsqrtf(group_sum(sum2(ss), gl) / (float)p.D + p.eps);
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < NSL; ++n) {
+        uint64_t ss = mul2(x[n][0], x[n][0]);
+#pragma unroll
+        for (int k = 1; k < V; ++k) ss = fma2(x[n][k], x[n][k], ss);
+        sum += sl[n].on ? sum2(ss) : 0.f;
+      }
+      const float r = rsqrtf(group_sum(sum, gl) * inv_d + p.eps);
       rstd = pair(r, r);
     }
 #pragma unroll
-    for (int n = 0; n < NSL; ++n)
-      if (live && sl[n].on) {
-        if (kind < 2) turn[n].apply(x[n], sl[n].j, half, norm);
-        if (norm) {
+    for (int n = 0; n < NSL; ++n) {
+      if (kind < 2) turn[n].apply(x[n], sl[n].j, half, norm);
+      if (norm) {
 #pragma unroll
-          for (int k = 0; k < V; ++k) x[n][k] = mul2(x[n][k], rstd);
-        }
-        store_pairs<T, V>(x[n], dst + sl[n].a, dst + sl[n].b);
+        for (int k = 0; k < V; ++k) x[n][k] = mul2(x[n][k], rstd);
       }
+      if (head < in.heads && sl[n].on) store_pairs<T, V>(x[n], to + sl[n].a, to + sl[n].b);
+    }
+  }
+    if (!more) break;
+    ++hblk;
+#pragma unroll
+    for (int h = 0; h < HPT; ++h)
+#pragma unroll
+      for (int n = 0; n < NSL; ++n) raw[h][n][0] = ahead[h][n][0], raw[h][n][1] = ahead[h][n][1];
   }
 }
 
@@ -401,19 +440,17 @@ __global__ void __launch_bounds__(kThreads) k_rotary_norm_bwd(const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gl = args.gl, l = lane & (gl - 1), sub = lane >> args.gl_shift, per = 32 >> args.gl_shift;
   const int half = p.rot / 2, nslots = p.D / (2 * V), hblocks = args.blocks[kind];
-  const HeadView &in = p.in[kind], &gr = p.grad[kind], &o = p.out[kind];
+  const HeadView in = pick(p.in, kind), gr = pick(p.grad, kind), o = pick(p.out, kind);
+  const void* wp = pick(p.w, kind);
   Slot<V> sl[NSL];
   uint64_t w[NSL][V], dw[NSL][V];
 #pragma unroll
   for (int n = 0; n < NSL; ++n) {
-    sl[n] = slot_of<V, INTER>(l + n * gl, nslots, half);
+    sl[n] = slot_of<V, INTER>(min(l + n * gl, nslots - 1), nslots, half);
+    sl[n].on = l + n * gl < nslots;
     float f[2 * V];
-#pragma unroll
-    for (int i = 0; i < 2 * V; ++i) f[i] = 0.f;
-    if (sl[n].on) {
-      load_weights<T, V>(p.w[kind], p.w_f32, sl[n].a, f);
-      load_weights<T, V>(p.w[kind], p.w_f32, sl[n].b, f + V);
-    }
+    load_weights<T, V>(wp, p.w_f32, sl[n].a, f);
+    load_weights<T, V>(wp, p.w_f32, sl[n].b, f + V);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       w[n][k] = pair(f[2 * k], f[2 * k + 1]);
@@ -422,7 +459,7 @@ __global__ void __launch_bounds__(kThreads) k_rotary_norm_bwd(const __grid_const
   }
   const int groups = args.groups[kind], units = p.batch * p.seq * groups;  // (the launcher keeps them below 2^30)
   const float inv_d = 1.f / (float)p.D;
-  const long long xstep = per * in.sh, gstep = per * gr.sh, dstep = per * o.sh;
+  const long long dstep = per * o.sh;
   for (int u = blk * kWarps + warp; u < units; u += args.nb[kind] * kWarps) {
     const int row = groups == 1 ? u : batch_of(u, groups, args.groups_inv[kind]), group = u - row * groups;
     const int b = batch_of(row, p.seq, args.seq_inv), s = row - b * p.seq;
@@ -431,12 +468,13 @@ __global__ void __launch_bounds__(kThreads) k_rotary_norm_bwd(const __grid_const
     Turn<V, INTER> turn[NSL];
 #pragma unroll
     for (int n = 0; n < NSL; ++n)
-      turn[n].load(p.cos_t, p.sin_t, in_table ? pos : 0, sl[n].j, half, sl[n].on, -1.f, nullptr);
+      turn[n].load(p.cos_t, p.sin_t, in_table ? pos : 0, sl[n].j, half, -1.f, nullptr);
     for (int hblk = group * args.inner; hblk < min(hblocks, (group + 1) * args.inner); ++hblk) {
-      const int head0 = hblk * args.hb + sub;
-      const T* xs = reinterpret_cast<const T*>(in.p) + b * in.sb + s * in.ss + head0 * in.sh;
-      const T* gs = reinterpret_cast<const T*>(gr.p) + b * gr.sb + s * gr.ss + head0 * gr.sh;
+      const int head0 = hblk * args.hb + sub;  // lanes and heads past the last as in the forward
+      const T* xs = reinterpret_cast<const T*>(in.p) + b * in.sb + s * in.ss;
+      const T* gs = reinterpret_cast<const T*>(gr.p) + b * gr.sb + s * gr.ss;
       T* ds = reinterpret_cast<T*>(const_cast<void*>(o.p)) + b * o.sb + s * o.ss + head0 * o.sh;
+      auto has = [&](int h) { return hblk * args.hb + h * per < in.heads; };
       if (!in_table) {  // a padded row: zeros, and no share of dw
 #pragma unroll
         for (int h = 0; h < HPT; ++h, ds += dstep)
@@ -447,38 +485,46 @@ __global__ void __launch_bounds__(kThreads) k_rotary_norm_bwd(const __grid_const
       }
       Pack<T, V> rx[HPT][NSL][2], rg[HPT][NSL][2];
 #pragma unroll
-      for (int h = 0; h < HPT; ++h, xs += xstep, gs += gstep)
+      for (int h = 0; h < HPT; ++h)
+        if (has(h)) {
+          const int head = min(head0 + h * per, in.heads - 1);
+          const T *xa = xs + head * in.sh, *ga = gs + head * gr.sh;
 #pragma unroll
-        for (int n = 0; n < NSL; ++n)
-          if (head0 + h * per < in.heads && sl[n].on) {
-            rx[h][n][0].load(xs + sl[n].a);
-            rx[h][n][1].load(xs + sl[n].b);
-            rg[h][n][0].load(gs + sl[n].a);
-            rg[h][n][1].load(gs + sl[n].b);
+          for (int n = 0; n < NSL; ++n) {
+            rx[h][n][0].load(xa + sl[n].a);
+            rx[h][n][1].load(xa + sl[n].b);
+            rg[h][n][0].load(ga + sl[n].a);
+            rg[h][n][1].load(ga + sl[n].b);
           }
+        }
 #pragma unroll
       for (int h = 0; h < HPT; ++h, ds += dstep) {
+        if (!has(h)) break;
         const bool live = head0 + h * per < in.heads;
-        uint64_t x[NSL][V], g[NSL][V], ss = pair(0.f, 0.f), sg = pair(0.f, 0.f);
+        uint64_t x[NSL][V], g[NSL][V];
+        float sx = 0.f, sxg = 0.f;
 #pragma unroll
-        for (int n = 0; n < NSL; ++n)
-          if (live && sl[n].on) {
-            to_pairs(rx[h][n][0], rx[h][n][1], x[n]);
-            to_pairs(rg[h][n][0], rg[h][n][1], g[n]);
-            turn[n].apply(g[n], sl[n].j, half, false);
+        for (int n = 0; n < NSL; ++n) {
+          to_pairs(rx[h][n][0], rx[h][n][1], x[n]);
+          to_pairs(rg[h][n][0], rg[h][n][1], g[n]);
+          turn[n].apply(g[n], sl[n].j, half, false);
+          uint64_t ss = mul2(x[n][0], x[n][0]), sg = mul2(x[n][0], mul2(g[n][0], w[n][0]));
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-              ss = fma2(x[n][k], x[n][k], ss);
-              sg = fma2(x[n][k], mul2(g[n][k], w[n][k]), sg);
-            }
+          for (int k = 1; k < V; ++k) {
+            ss = fma2(x[n][k], x[n][k], ss);
+            sg = fma2(x[n][k], mul2(g[n][k], w[n][k]), sg);
           }
-        const float sx = group_sum(sum2(ss), gl), sxg = group_sum(sum2(sg), gl);
+          sx += sl[n].on ? sum2(ss) : 0.f;
+          sxg += sl[n].on ? sum2(sg) : 0.f;
+        }
+        sx = group_sum(sx, gl);
+        sxg = group_sum(sxg, gl);
         const float r = rsqrtf(sx * inv_d + p.eps);
         const float m = -(r * sxg * inv_d) * r * r;  // -rstd^2 mean(w g h): dx = rstd w g + m x
         const uint64_t r2 = pair(r, r), m2 = pair(m, m);
+        if (live) {
 #pragma unroll
-        for (int n = 0; n < NSL; ++n)
-          if (live && sl[n].on) {
+          for (int n = 0; n < NSL; ++n) {
             uint64_t d[V];
 #pragma unroll
             for (int k = 0; k < V; ++k) {
@@ -486,8 +532,9 @@ __global__ void __launch_bounds__(kThreads) k_rotary_norm_bwd(const __grid_const
               d[k] = fma2(x[n][k], m2, mul2(gr2, w[n][k]));
               dw[n][k] = fma2(gr2, x[n][k], dw[n][k]);
             }
-            store_pairs<T, V>(d, ds + sl[n].a, ds + sl[n].b);
+            if (sl[n].on) store_pairs<T, V>(d, ds + sl[n].a, ds + sl[n].b);
           }
+        }
       }
     }
   }
@@ -585,6 +632,10 @@ cudaError_t launch_fwd(const RotaryParams& p, cudaStream_t s) {
   const long long rows = (long long)p.batch * p.seq;
   long long hblocks = 0;
   for (int i = 0; i < 3; ++i) hblocks += a.blocks[i] = (p.in[i].heads + a.hb - 1) / a.hb;
+  // as many steps in a warp as leave the GPU full
+  a.inner = HPT == 1 ? 1 : (int)std::max<long long>(1, std::min<long long>(hblocks, rows * hblocks / (148 * 32)));
+  hblocks = 0;
+  for (int i = 0; i < 3; ++i) hblocks += a.groups[i] = (a.blocks[i] + a.inner - 1) / a.inner;
   a.wh_shift = hblocks >= 4 ? 2 : hblocks >= 2 ? 1 : 0;
   const int wh = 1 << a.wh_shift;
   a.seq_inv = inverse_of(rows, p.seq);
@@ -595,12 +646,11 @@ cudaError_t launch_fwd(const RotaryParams& p, cudaStream_t s) {
                   dim3(kThreads), 0, s, a);
 }
 
-template <typename T, int HPT, bool INTER>
+template <typename T, bool MANY, bool INTER>
 cudaError_t wide_fwd(const RotaryParams& p, cudaStream_t s) {
-  constexpr int VM = 16 / (int)sizeof(T);
-  if (p.append)
-    return p.w[0] ? launch_fwd<T, VM, 1, HPT, kAppendNorm, INTER>(p, s) : launch_fwd<T, VM, 1, HPT, kAppend, INTER>(p, s);
-  return p.w[0] ? launch_fwd<T, VM, 1, HPT, kNorm, INTER>(p, s) : launch_fwd<T, VM, 1, HPT, kPlain, INTER>(p, s);
+  constexpr int VM = 16 / (int)sizeof(T), A = MANY ? kSteps : 1, N = MANY ? kStepsNorm : 1;
+  if (p.append) return p.w[0] ? launch_fwd<T, VM, 1, N, kAppendNorm, INTER>(p, s) : launch_fwd<T, VM, 1, A, kAppend, INTER>(p, s);
+  return p.w[0] ? launch_fwd<T, VM, 1, N, kNorm, INTER>(p, s) : launch_fwd<T, VM, 1, A, kPlain, INTER>(p, s);
 }
 
 template <typename T>
@@ -611,8 +661,8 @@ cudaError_t forward_t(const RotaryParams& p, cudaStream_t s) {
     const long long heads = (long long)p.batch * p.seq * (p.in[0].heads + p.in[1].heads + p.in[2].heads);
     const int per = 32 / lanes_of(p.D / (2 * VM));
     const bool many = heads >= 148ll * 64 * per;
-    if (p.interleaved) return many ? wide_fwd<T, 4, true>(p, s) : wide_fwd<T, 1, true>(p, s);
-    return many ? wide_fwd<T, 4, false>(p, s) : wide_fwd<T, 1, false>(p, s);
+    if (p.interleaved) return many ? wide_fwd<T, true, true>(p, s) : wide_fwd<T, false, true>(p, s);
+    return many ? wide_fwd<T, true, false>(p, s) : wide_fwd<T, false, false>(p, s);
   }
   auto narrow = [&](auto inter) {
     constexpr bool I = decltype(inter)::value;

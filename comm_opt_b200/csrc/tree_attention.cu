@@ -2,21 +2,30 @@
 //
 // For one (sequence, KV head) the rows are all drafted tokens of all its query heads, r = t * G + g, so every cache
 // byte is read once per 256 rows. A CTA owns NT row tiles of 128 rows (NT = 2 above 128 rows) and walks 128-token
-// tiles of the cache with the online softmax
+// tiles of the cache, 64 tokens a step, with the online softmax
 //   S = Q K^T;  m' = max(m, row max);  P = 2^((S - m') c);  l = l 2^((m - m') c) + sum P;  O = O 2^((m - m') c) + P V
 // with c = scale log2(e). A row tile's row is one TMEM lane and one thread of a softmax warpgroup, so maxima and
 // sums need no shuffles. Roles: one warp loads K tiles, one V tiles (8 pages of 16 tokens as 64-column TMA boxes
 // whose 128-byte swizzle makes them tcgen05 operands: K is K-major, V N-major), one issues the MMAs, NT warpgroups do
-// the softmax. S is written by the tensor cores into one of two TMEM buffers, P goes back over it in 16 bits and is
-// the A operand of P V straight from TMEM; O stays in TMEM. The two buffers belong to the two row tiles (NT = 2) or to
-// alternate KV tiles (NT = 1), so the tensor cores work on one while the other is in the softmax.
-// O is rescaled only when a row's maximum rose by more than 2^8 (P stays below 2^8, far inside the 16-bit types;
-// O / l is the same number), which after the first tiles hardly happens.
+// the softmax. S is written by the tensor cores into one of a row tile's two TMEM buffers, P goes back over it in 16 bits
+// and is the A operand of P V straight from TMEM; O stays in TMEM. Q K^T of the next step runs while the softmax works
+// on this one, which is what two buffers of 64 columns per row tile are for (one of 128 left the softmax waiting 1 us a
+// tile for its scores). O is rescaled only where a row's maximum rose by more than 2^8 (P stays below 2^8, far inside the
+// 16-bit types; O / l is the same number), which after the first tiles hardly happens.
 //
-// Work is cut into equal shares of the flattened (sequence, KV head, tile) space by the sequences' actual lengths, so
-// ragged batches and few long sequences both fill the GPU; the RB CTAs that hold the row blocks of one share walk
-// it side by side and meet each other's cache tiles in L2. A (sequence, head) cut between shares leaves
-// unnormalised partials (at most two per CTA) that a second kernel joins in the shares' order.
+// Work is cut into equal shares of the flattened (sequence, KV head, tile) space by the sequences' actual lengths,
+// each (sequence, KV head) charged two tiles for its start and end, so ragged batches and few long sequences both fill
+// the GPU; the RB CTAs that hold the row blocks of one share walk it side by side and meet each other's cache tiles in
+// L2. A (sequence, head) cut between shares leaves unnormalised partials (at most two per CTA) that a second kernel,
+// launched early, joins in the shares' order.
+//
+// Bounds, measured on one B200 at 4 x 64 drafted tokens over 32k, 64 / 8 heads of 128 (0.55 GB, 275 GFLOP): 287 us, 0.96
+// PFLOP/s. Without the softmax the same walk takes 222 us, of which Q K^T 97 us: M = 128, N = 64 from shared memory reads
+// 6 KB per 32 cycles of arithmetic and the memory gives 128 bytes a cycle, but 128 columns do not fit beside O twice.
+// Exponentials on the FMA pipe (a degree-5 polynomial for 2 to 4 of 8), 16 softmax warps of 16 rows each (16x256b TMEM
+// accesses) and 128-column steps were all measured and no faster (288 - 303, 306, 305 us).
+// Small: 8 drafted tokens over 1k, 32 / 8 heads: 10.8 us, latencies (lengths, page indices and first pages 3.2, one tile
+// 1.5, output 1, the join 3). 8 x 16 over up to 2k, 64 / 8 heads (38 MB): 21.5 us.
 //
 // What a row does not see must not reach it, even when it is not finite: scores are replaced, not added to; slots past
 // the last token are zeroed in the V tile; a non-finite component of a drafted token's v is zeroed there too, and
@@ -76,24 +85,43 @@ __device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// D[tmem] (+)= A[tmem] * B[smem], 16-bit A packed two components to a column
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// The MMA warp runs its loop as a whole and one elected lane issues: what feeds the instructions is then the same in all
+// lanes and stays in uniform registers (behind a branch on the lane, moving it there took 100 cycles per MMA).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
+}
+// Shared-memory matrix descriptors as (low, high) words; a step along the operand adds its bytes / 16 to the low word.
+// K-major: 128-byte swizzle, 8-row groups 1024 bytes apart. N-major: 64-column groups `lbo` bytes apart, 8-row groups 1024.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | (lbo >> 4) << 16; }
+// D[tmem] (+)= A[smem] * B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "mov.b64 da, {%1, %6};\n\tmov.b64 db, {%2, %6};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(leader), "n"(kDescHigh)
       : "memory");
 }
-// N-major operand, 128-byte swizzle: 64-column groups `lbo` bytes apart, 8-row groups 1024 bytes apart
-__device__ __forceinline__ uint64_t desc_n_sw128(uint32_t addr, uint32_t lbo) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr >> 4) & 0x3FFFu);
-  d |= (uint64_t)(lbo >> 4) << 16;
-  d |= (uint64_t)(1024u >> 4) << 32;
-  d |= (uint64_t)1u << 46;
-  d |= (uint64_t)2u << 61;
-  return d;
+// D[tmem] (+)= A[tmem] * B[smem], 16-bit A packed two components to a column
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "mov.b64 db, {%2, %6};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(leader), "n"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+      "r"(leader)
+      : "memory");
 }
 constexpr uint32_t kBNMajor = 1u << 16;  // instruction descriptor: B is N-major
 constexpr uint32_t kNegateA = 1u << 13;  // instruction descriptor: A enters with its sign changed
@@ -106,9 +134,10 @@ __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.
 __device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
+// NaN if any is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -167,13 +196,22 @@ __device__ __forceinline__ void quad_transpose(uint4 (&v)[4], int lane) {
   swap(v[1], v[3], 2);
 }
 
-// Bounded wait of a whole warp, one verdict for all lanes (and reconverged: the TMEM accesses that follow need it).
-// Every waiter of a barrier sees every phase of it in turn, so the parity is never ambiguous.
+// Bounded wait of a whole warp, one verdict for all lanes (and reconverged: the TMEM accesses that follow need it). The
+// timer and the failure flag are only looked at every 64 tries. Every waiter of a barrier sees every phase of it in turn,
+// so the parity is never ambiguous.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* fail) {
-  const bool good = mbar_wait(bar, parity, kTimeout) && *fail == 0;
-  if (__all_sync(0xffffffffu, good)) return true;
-  *fail = 1;
-  return false;
+  uint64_t t0 = 0;
+  for (uint32_t tries = 1;; ++tries) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((tries & 63u) == 0) {
+      const uint64_t t = globaltimer();
+      if (t0 == 0) t0 = t;
+      if (__any_sync(0xffffffffu, t - t0 > kTimeout || *fail != 0)) {
+        *fail = 1;
+        return false;
+      }
+    }
+  }
 }
 
 // ----------------------------------------------------------------------------- geometry
@@ -184,10 +222,12 @@ struct Geo {
   static constexpr int HALF_BYTES = kTile * 128;          // 64 columns of a tile
   static constexpr int TILE_BYTES = kTile * D * 2;        // Q, K or V tile
   static constexpr int KS = 3, VS = NT == 2 ? 2 : 3;      // ring stages (227 KB per CTA at D = 128)
-  static constexpr int WARPS = 4 * NT + 3;
+  static constexpr int WARPS = 4 * NT + 4;                // 4 softmax warps per row tile, 2 loading, 1 issuing MMAs, 1 idle
   static constexpr int THREADS = WARPS * 32;
   static constexpr int SMEM = 1024 + NT * TILE_BYTES + (KS + VS) * TILE_BYTES + 256 + (3 * kMaxBatch + 1) * 4;
-  static constexpr uint32_t S0 = 0, S1 = 128, O0 = 256;   // TMEM columns
+  static constexpr int STEP = 64;                         // tokens of a score buffer: two per row tile fit beside O
+  static constexpr int PER = kTile / STEP;                // steps of a tile
+  static constexpr uint32_t O0 = 256;                     // TMEM columns: score buffers [tile][2] of STEP, then O of each tile
 };
 
 struct alignas(64) TreeArgs {
@@ -255,6 +295,11 @@ struct Segment {
   int b, kvh, t0, t1, nt;
   bool first;  // of the (sequence, KV head) that holds the share's first position (partial slot 0, else 1)
 };
+// steps of a piece: STEP tokens each, up to the last one that holds a token
+template <int STEP>
+__device__ __forceinline__ int steps_of(const Segment& s, int len) {
+  return (s.t1 - s.t0) * (kTile / STEP) - (s.t1 == s.nt ? (s.nt * kTile - len) / STEP : 0);
+}
 struct Walk {
   const int* cum;
   int batch, nkv, g, beg, end;
@@ -301,12 +346,11 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
   uint64_t* k_empty = k_full + C::KS;
   uint64_t* v_full = k_empty + C::KS;
   uint64_t* v_empty = v_full + C::VS;
-  uint64_t* s_full = v_empty + C::VS;  // [2] scores of a buffer are in TMEM
-  uint64_t* p_low = s_full + 2;        // [2] weights of a buffer's first half are in TMEM
-  uint64_t* p_ready = p_low + 2;       // [2] and those of the second
-  uint64_t* o_done = p_ready + 2;      // [NT] one more P V of a row tile has completed
-  uint64_t* q_ready = o_done + 2;      // [NT] query tile staged
-  uint64_t* drain = q_ready + 2;
+  uint64_t* s_full = v_empty + C::VS;    // [NT][2] scores of a buffer are in TMEM
+  uint64_t* p_ready = s_full + 2 * NT;   // [NT][2] and its weights
+  uint64_t* o_done = p_ready + 2 * NT;   // [NT] one more P V of a row tile has completed
+  uint64_t* q_ready = o_done + NT;       // [NT] query tile staged
+  uint64_t* drain = q_ready + NT;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* s_fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_odd = reinterpret_cast<int*>(tmem_slot + 2);  // a drafted v of this segment is not finite
@@ -317,13 +361,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::KS; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
     for (int i = 0; i < C::VS; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_low[i], 4);
-      mbar_init(&p_ready[i], 4);
-      mbar_init(&o_done[i], 1);
-      mbar_init(&q_ready[i], 4);
-    }
+    for (int i = 0; i < 2 * NT; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_ready[i], 4);
+    for (int i = 0; i < NT; ++i) mbar_init(&o_done[i], 1), mbar_init(&q_ready[i], 4);
     mbar_init(drain, 1);
     *s_fail = 0;
     *s_odd = 0;
@@ -383,66 +422,65 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     if (!okay)  // copies in flight must land before the CTA's memory is given back
       for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(&full[i % stages], (i / stages) & 1, kTimeout);
   } else if (warp == WM) {
-    // ------------------------------------------------ MMAs: S(n) = Q K^T into buffer n & 1, O += P(n) V
-    if (lane == 0) {
-      const uint32_t id_qk = idesc_f16(128, kTile, BF16) | (p.scale < 0.f ? kNegateA : 0u);
-      constexpr uint32_t id_pv = idesc_f16(128, D, BF16) | kBNMajor;
-      int n0 = 0, i0 = 0, seg = 0;  // row-tile steps, KV tiles and segments before this segment
-      bool okay = true;
-      while (okay && walk.next(sg)) {
-        for (int q = 0; q < NT && okay; ++q)
-          if (!mbar_wait(&q_ready[q], seg & 1, kTimeout) || *s_fail) okay = false;
-        if (!okay) break;
-        const int steps = (sg.t1 - sg.t0) * NT;
-        auto qk = [&](int m) {
-          const int i = i0 + m / NT, st = i % C::KS, tile = m % NT;
-          if (!mbar_wait(&k_full[st], (i / C::KS) & 1, kTimeout) || *s_fail) return false;
+    // ------------------------------------------------ MMAs: step s of row tile q is S[q][s & 1] = Q K^T, O[q] += P V
+    const uint32_t leader = elect_one();
+    const uint32_t id_qk = idesc_f16(128, C::STEP, BF16) | (p.scale < 0.f ? kNegateA : 0u);
+    constexpr uint32_t id_pv = idesc_f16(128, D, BF16) | kBNMajor;
+    const uint32_t q_desc = desc_low(smem_addr(sQ), 16), k_desc = desc_low(smem_addr(sK), 16);
+    const uint32_t v_desc = desc_low(smem_addr(sV), C::HALF_BYTES);
+    int n0 = 0, i0 = 0, seg = 0;  // steps, KV tiles and segments before this segment
+    bool okay = true;
+    while (okay && walk.next(sg)) {
+      for (int q = 0; q < NT && okay; ++q) okay = warp_wait(&q_ready[q], seg & 1, s_fail);
+      const int steps = steps_of<C::STEP>(sg, lens.at(p, sg.b).len);
+      auto qk = [&](int s, int q) {
+        const int i = i0 + s / C::PER, st = i % C::KS, n = n0 + s;
+        if (q == 0 && s % C::PER == 0) {
+          if (!warp_wait(&k_full[st], (i / C::KS) & 1, s_fail)) return false;
           tc_fence_after();
-          const uint32_t a = smem_addr(sQ + tile * C::TILE_BYTES), b = smem_addr(sK + st * C::TILE_BYTES);
-          const uint32_t d = tmem + (((n0 + m) & 1) ? C::S1 : C::S0);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk / 4) * C::HALF_BYTES + (kk % 4) * 32;
-            mma_f16(d, desc_k_sw128(a + off), desc_k_sw128(b + off), id_qk, kk > 0);
-          }
-          mma_commit(&s_full[(n0 + m) & 1]);
-          if (tile == NT - 1) mma_commit(&k_empty[st]);
-          return true;
-        };
-        okay = qk(0) && (steps < 2 || qk(1));
-        for (int m = 0; m < steps && okay; ++m) {
-          const int n = n0 + m, i = i0 + m / NT, st = i % C::VS, tile = m % NT;
-          const uint32_t a = tmem + ((n & 1) ? C::S1 : C::S0), b = smem_addr(sV + st * C::TILE_BYTES);
-          const uint32_t d = tmem + C::O0 + tile * D;
-          okay = mbar_wait(&p_low[n & 1], (n >> 1) & 1, kTimeout) && mbar_wait(&v_full[st], (i / C::VS) & 1, kTimeout) &&
-                 *s_fail == 0;
-          if (!okay) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < kTile / 32; ++kk)
-            mma_ts(d, a + kk * 8, desc_n_sw128(b + kk * 2048, C::HALF_BYTES), id_pv, m >= NT || kk > 0);
-          okay = mbar_wait(&p_ready[n & 1], (n >> 1) & 1, kTimeout) && *s_fail == 0;
-          if (!okay) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = kTile / 32; kk < kTile / 16; ++kk)
-            mma_ts(d, a + kk * 8, desc_n_sw128(b + kk * 2048, C::HALF_BYTES), id_pv, 1u);
-          mma_commit(&o_done[tile]);
-          if (tile == NT - 1) mma_commit(&v_empty[st]);
-          if (m + 2 < steps) okay = qk(m + 2);
         }
-        n0 += steps;
-        i0 += sg.t1 - sg.t0;
-        ++seg;
+        const uint32_t a = q_desc + q * (C::TILE_BYTES >> 4);
+        const uint32_t b = k_desc + (st * C::TILE_BYTES + s % C::PER * (C::STEP * 128) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk / 4 * C::HALF_BYTES + kk % 4 * 32) >> 4;
+          mma_ss(tmem + (2 * q + (n & 1)) * C::STEP, a + off, b + off, id_qk, kk > 0, leader);
+        }
+        commit(&s_full[2 * q + (n & 1)], leader);
+        if (q == NT - 1 && (s % C::PER == C::PER - 1 || s + 1 == steps)) commit(&k_empty[st], leader);
+        return true;
+      };
+      for (int s = 0; s < min(steps, 2) && okay; ++s)
+        for (int q = 0; q < NT && okay; ++q) okay = qk(s, q);
+      for (int s = 0; s < steps && okay; ++s) {
+        const int n = n0 + s, i = i0 + s / C::PER, st = i % C::VS;
+        const uint32_t b = v_desc + (st * C::TILE_BYTES + s % C::PER * (C::STEP * 128) >> 4);
+#pragma unroll
+        for (int q = 0; q < NT; ++q) {
+          okay = okay && warp_wait(&p_ready[2 * q + (n & 1)], (n >> 1) & 1, s_fail);
+          if (q == 0 && s % C::PER == 0) okay = okay && warp_wait(&v_full[st], (i / C::VS) & 1, s_fail);
+          if (!okay) break;
+          tc_fence_after();
+          const uint32_t a = tmem + (2 * q + (n & 1)) * C::STEP;
+#pragma unroll
+          for (int kk = 0; kk < C::STEP / 16; ++kk)
+            mma_ts(tmem + C::O0 + q * D, a + kk * 8, b + kk * (2048 >> 4), id_pv, s > 0 || kk > 0, leader);
+          commit(&o_done[q], leader);
+          if (q == NT - 1 && (s % C::PER == C::PER - 1 || s + 1 == steps)) commit(&v_empty[st], leader);
+          if (s + 2 < steps) okay = qk(s + 2, q);
+        }
       }
-      if (!okay) {  // MMAs in flight must end before their memory is given back
-        *s_fail = 1;
-        mma_commit(drain);
-        mbar_wait(drain, 0, kTimeout);
-      }
+      n0 += steps;
+      i0 += sg.t1 - sg.t0;
+      ++seg;
+    }
+    if (!okay) {  // MMAs in flight must end before their memory is given back
+      *s_fail = 1;
+      commit(drain, leader);
+      mbar_wait(drain, 0, kTimeout);
     }
     __syncwarp();
-  } else {
+  } else if (warp < WK) {
     // ------------------------------------------------ softmax and epilogue: warpgroup `tile`, thread = row
     const int tile = warp >> 2, wq = warp & 3;
     const uint32_t lanes = (uint32_t)(wq * 32) << 16;
@@ -489,89 +527,89 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
         if (nodes < 64) bits &= (1ull << nodes) - 1ull;
       }
       float m = -INFINITY, l = 0.f;
-      for (int t = cur.t0; t < cur.t1; ++t) {
-        const int j = t - cur.t0, n = n0 + (NT == 1 ? j : 2 * j + tile), i = i0 + j;
-        const uint32_t sbuf = tmem + lanes + ((n & 1) ? C::S1 : C::S0), obuf = tmem + lanes + C::O0 + tile * D;
-        const int s0 = t * kTile;
-        const bool tail = s0 + kTile > sl.ctx;
-        okay = warp_wait(&s_full[n & 1], (n >> 1) & 1, s_fail);
+      const int steps = steps_of<C::STEP>(cur, sl.len);
+      const uint32_t obuf = tmem + lanes + C::O0 + tile * D;
+      for (int st = 0; st < steps; ++st) {
+        const int n = n0 + st, i = i0 + st / C::PER, s0 = cur.t0 * kTile + st * C::STEP;
+        const uint32_t sbuf = tmem + lanes + (2 * tile + (n & 1)) * C::STEP;
+        const bool tail = s0 + C::STEP > sl.ctx;
+        okay = warp_wait(&s_full[2 * tile + (n & 1)], (n >> 1) & 1, s_fail);
         if (!okay) break;
         tc_fence_after();
-        if (t + 1 == cur.t1) {  // every Q K^T of this piece has completed: the next piece's queries may be staged
+        if (st + 1 == steps) {  // every Q K^T of this piece has completed: the next piece's queries may be staged
           have = walk.next(sg);
           if (have) stage_q(sg);
         }
         if (tail && tile == 0) {
-          // thread = slot of the V tile: zero it past the last token, and zero non-finite components of drafted tokens
-          const int st = i % C::VS, slot = s0 + (int)threadIdx.x;
-          okay = warp_wait(&v_full[st], (i / C::VS) & 1, s_fail);
+          // 128 / STEP threads per slot of the step's V rows: zero them past the last token, and zero non-finite components
+          // of drafted tokens
+          constexpr int CELLS = C::HALVES * 8 * C::STEP / 128;
+          const int vs = i % C::VS, at = threadIdx.x % C::STEP, sr = st % C::PER * C::STEP + at, slot = s0 + at;
+          const int part = threadIdx.x / C::STEP;
+          okay = warp_wait(&v_full[vs], (i / C::VS) & 1, s_fail);
           if (!okay) break;
           if (slot >= sl.ctx) {
-            uint8_t* vr = sV + st * C::TILE_BYTES + threadIdx.x * 128;
+            uint8_t* vr = sV + vs * C::TILE_BYTES + sr * 128;
+            auto cell = [&](int k) {  // this thread's part of the row, in an order free of bank conflicts
+              const int e = part * CELLS + k;
+              return reinterpret_cast<uint4*>(vr + e / 8 * C::HALF_BYTES + (((e + lane) & 7) << 4));
+            };
+            if (slot >= sl.len) {
 #pragma unroll
-            for (int h = 0; h < C::HALVES; ++h) {
-              uint4 v[8];
-              auto cell = [&](int k) { return reinterpret_cast<uint4*>(vr + h * C::HALF_BYTES + (((k + lane) & 7) << 4)); };
-              if (slot >= sl.len) {
+              for (int k = 0; k < CELLS; ++k) *cell(k) = make_uint4(0, 0, 0, 0);
+            } else {
+              uint4 v[CELLS];
+              uint32_t odd = 0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) *cell(k) = make_uint4(0, 0, 0, 0);
-              } else {
-                uint32_t odd = 0;
+              for (int k = 0; k < CELLS; ++k) v[k] = *cell(k);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = *cell(k);
+              for (int k = 0; k < CELLS; ++k) odd |= drop_odd<T>(v[k]);
+              if (odd) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) odd |= drop_odd<T>(v[k]);
-                if (odd) {
-#pragma unroll
-                  for (int k = 0; k < 8; ++k) *cell(k) = v[k];
-                  *s_odd = 1;
-                }
+                for (int k = 0; k < CELLS; ++k) *cell(k) = v[k];
+                *s_odd = 1;
               }
             }
           }
           fence_proxy_async();
         }
+        constexpr int G = C::STEP / 32;
+        uint32_t w[G / 2][32];
         if (warp_live) {
-          uint32_t s[4][32];
+          uint32_t s[G][32];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tmem_ld32(sbuf + 32 * k, s[k]);
+          for (int k = 0; k < G; ++k) tmem_ld32(sbuf + 32 * k, s[k]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tmem_landed(s[k]);
-          if (tail) {
+          for (int k = 0; k < G; ++k) tmem_landed(s[k]);
+          if (tail) {  // scores of slots that the row does not see
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int node = s0 + 32 * k - sl.ctx;  // drafted token of the group's first column
-              const uint32_t see = node >= 64 ? 0u
-                                   : node >= 0 ? (uint32_t)(bits >> node)
-                                   : node > -32 ? (uint32_t)(bits << -node) | ((1u << -node) - 1u)
-                                                : 0xffffffffu;
+            for (int k = 0; k < G; k += 2) {
+              const int node = s0 + 32 * k - sl.ctx;  // drafted token of the 64 columns' first
+              const unsigned long long see = node >= 64   ? 0ull
+                                             : node >= 0  ? bits >> node
+                                             : node > -64 ? (bits << -node) | ((1ull << -node) - 1ull)
+                                                          : ~0ull;
 #pragma unroll
-              for (int x = 0; x < 32; ++x)
-                if (!((see >> x) & 1u)) s[k][x] = 0xff800000u;
+              for (int x = 0; x < 64; ++x)
+                if (!((see >> x) & 1ull)) s[k + x / 32][x % 32] = 0xff800000u;
             }
           }
-          float mx[8];
+          float mx[4] = {m, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            auto f = [&](int x) { return __uint_as_float(s[k][x]); };
-            mx[2 * k] = max3(f(0), f(1), f(2));
-            mx[2 * k + 1] = max3(f(16), f(17), f(18));
+          for (int x = 0; x < 32; x += 4)
 #pragma unroll
-            for (int x = 3; x < 15; x += 2) {
-              mx[2 * k] = max3(mx[2 * k], f(x), f(x + 1));
-              mx[2 * k + 1] = max3(mx[2 * k + 1], f(16 + x), f(17 + x));
+            for (int k = 0; k < G; ++k) {
+              mx[k % 2 * 2] = max3(mx[k % 2 * 2], __uint_as_float(s[k][x]), __uint_as_float(s[k][x + 1]));
+              mx[k % 2 * 2 + 1] = max3(mx[k % 2 * 2 + 1], __uint_as_float(s[k][x + 2]), __uint_as_float(s[k][x + 3]));
             }
-            mx[2 * k] = max3(mx[2 * k], f(15), f(31));
-          }
-          const float mn = fmaxf(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), mx[6]), fmaxf(mx[7], m));
-          if (j == 0) {
-            m = mn;
-          } else if (__any_sync(0xffffffffu, (mn - m) * c > 8.f)) {
-            // rescale this warp's rows of O, which the previous P V has finished
-            const float f = mn == m ? 1.f : ex2((m - mn) * c);
-            m = mn;
-            l *= f;
-            okay = warp_wait(&o_done[tile], (i - 1) & 1, s_fail);
+          float mn = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+          if (mn == INFINITY) mn = __uint_as_float(0x7fc00000u);  // inf - inf
+          const bool rise = st == 0 || !((mn - m) * c <= 8.f);
+          const float f = !rise || mn == m ? 1.f : ex2((m - mn) * c);
+          if (rise) m = mn;  // (by row: no row's result depends on another's)
+          l *= f;
+          if (st > 0 && __any_sync(0xffffffffu, rise)) {  // rescale rows of O, which the previous P V has finished
+            okay = warp_wait(&o_done[tile], (n - 1) & 1, s_fail);
             if (!okay) break;
             tc_fence_after();
 #pragma unroll 1
@@ -588,47 +626,36 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
           const uint64_t c2 = pair(c, c), mu2 = pair(-mu, -mu);
           uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            uint32_t w[32];
-#pragma unroll
-            for (int x = 0; x < 32; ++x) {
-              const int e = 2 * x;  // column 64 k + e
-              float a, b;
-              unpair(fma2(pair(__uint_as_float(s[2 * k + e / 32][e % 32]), __uint_as_float(s[2 * k + e / 32][e % 32 + 1])), c2, mu2), a, b);
-              a = ex2(a);
-              b = ex2(b);
-              sum[x & 1] = add2(sum[x & 1], pair(a, b));
-              w[x] = pack2<T>(a, b);
-            }
-            if (k == 0 && j > 0) {  // the previous P V has long ended; seeing its phase keeps this warp's parity in step
-              okay = warp_wait(&o_done[tile], (i - 1) & 1, s_fail);
-              if (!okay) break;
-            }
-            tmem_st32(sbuf + 32 * k, w);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(k ? &p_ready[n & 1] : &p_low[n & 1]);
+          for (int x = 0; x < 16 * G; ++x) {
+            float a, b;
+            unpair(fma2(pair(__uint_as_float(s[x / 16][x % 16 * 2]), __uint_as_float(s[x / 16][x % 16 * 2 + 1])), c2, mu2), a, b);
+            a = ex2(a);
+            b = ex2(b);
+            sum[x & 1] = add2(sum[x & 1], pair(a, b));
+            w[x / 32][x % 32] = pack2<T>(a, b);
           }
-          if (!okay) break;
-          float a, b;
-          unpair(add2(sum[0], sum[1]), a, b);
-          l += a + b;
-        } else {
-          if (j > 0) {
-            okay = warp_wait(&o_done[tile], (i - 1) & 1, s_fail);
-            if (!okay) break;
-          }
-          if (lane == 0) mbar_arrive(&p_low[n & 1]), mbar_arrive(&p_ready[n & 1]);
+          l += sum2(add2(sum[0], sum[1]));
         }
+        if (st > 0) {  // the previous P V has long ended; seeing its phase keeps this warp's parity in step
+          okay = warp_wait(&o_done[tile], (n - 1) & 1, s_fail);
+          if (!okay) break;
+        }
+        if (warp_live) {
+#pragma unroll
+          for (int k = 0; k < G / 2; ++k) tmem_st32(sbuf + 32 * k, w[k]);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[2 * tile + (n & 1)]);
       }
       if (!okay) break;
       if (have) q_staged();
-      const int tiles = cur.t1 - cur.t0, last = i0 + tiles - 1;
-      okay = warp_wait(&o_done[tile], last & 1, s_fail);
+      const int tiles = cur.t1 - cur.t0;
+      okay = warp_wait(&o_done[tile], (n0 + steps - 1) & 1, s_fail);
       if (!okay) break;
       tc_fence_after();
-      n0 += NT * tiles;
+      n0 += steps;
       i0 += tiles;
       const bool whole = tiles == cur.nt;
       const bool odd = *reinterpret_cast<volatile int*>(s_odd) != 0;  // (kept set: a re-check, not a result)
@@ -716,7 +743,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(128) k_tree_join(const __grid_constant__ TreeArgs args) {
   using C = Geo<D, NT>;
-  constexpr int PARTS = D / 16, kBatch = 4;
+  constexpr int PARTS = D / 16, kBatch = 8;
   const TreeAttnParams& p = args.p;
   const int lane = threadIdx.x & 31;
   const int b = blockIdx.z, kvh = blockIdx.y;

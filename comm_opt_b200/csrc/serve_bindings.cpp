@@ -72,6 +72,9 @@ Tables tables(const Tensor& cos_t, const Tensor& sin_t, int64_t D, const Tensor&
   COB_CHECK(rot >= 2 && rot <= D, "rotary_dim (2 x the tables' columns) must be between 2 and head_dim, got ", rot,
             " for head_dim ", D);
   COB_CHECK(!cos_t.requires_grad() && !sin_t.requires_grad(), "cos and sin are constants: no gradient is formed");
+  // rows of a multiple of four angles are read four at a time
+  for (const auto* t : {&cos_t, &sin_t})
+    COB_CHECK(cos_t.size(1) % 4 || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "cos and sin must be 16-byte aligned");
   return {(int)cos_t.size(0), (int)rot};
 }
 
@@ -307,8 +310,8 @@ void cache_ok(const Tensor& k, const Tensor& v, const Tensor& bt, const Tensor& 
   COB_CHECK(k.size(0) == v.size(0), "k_cache and v_cache must have the same number of blocks");
   COB_CHECK(k.size(0) * nkv * 16 < (1ll << 31), "a cache holds at most 2^31 - 1 head rows");
   dense(bt, "block_tables", torch::kInt, ref);
-  COB_CHECK(bt.dim() == 2 && bt.size(0) == batch && bt.size(1) >= 1 && bt.size(1) < (1 << 27),
-            "block_tables must be [batch, max_blocks]");
+  COB_CHECK(bt.dim() == 2 && bt.size(0) == batch && bt.size(1) >= 1 && bt.size(1) <= (1 << 26),
+            "block_tables must be [batch, max_blocks], at most 2^26 pages a sequence");
 }
 
 void lens_ok(const Tensor& t, const char* n, int64_t batch, const Tensor& ref) {

@@ -84,8 +84,9 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, cos, sin, eps: float = 1
     (shapes, positions and tables as in `rotary`); the norms are over each head's D components, their weights [D] of
     the operands' type or fp32. fp32 inside, one rounding at the end.
 
-    Differentiable in q, k and both weights (`qk_norm_rotary_backward` is the same gradient as a plain call, e.g. to
-    capture it in a CUDA graph)."""
+    Differentiable in q, k and both weights. `qk_norm_rotary_backward` is the same gradient as a plain call: it can be
+    captured in a CUDA graph whatever else is alive, which torch allows for autograd only while no eager graph of the same
+    leaves is."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or
                                     k_weight.requires_grad):
         return native().qk_norm_rotary_autograd(q, k, q_weight, k_weight, positions, cos, sin, float(eps), bool(interleaved))

@@ -732,6 +732,85 @@ def test_programmatic_launch_keeps_the_results(cuda):
     assert all(torch.equal(s[n], w) for n, w in zip(("ids", "o", "kc", "vc"), want))
 
 
+def test_caches_past_32_bit_offsets(cuda):
+    """Pages whose elements lie beyond 2^31: appended to and attended like the same pages of a small cache."""
+    g = gen(cuda, 21)
+    nkv, D, B, T = 8, 128, 2, 5
+    blocks = 2 ** 31 // (nkv * 16 * D) + 40
+    kc = torch.zeros(blocks, nkv, 16, D, device=cuda, dtype=torch.bfloat16)
+    vc = torch.zeros_like(kc)
+    far = torch.arange(blocks - 32, blocks, device=cuda).view(B, 16).to(torch.int32)
+    near = torch.arange(32, device=cuda).view(B, 16).to(torch.int32)
+    ks, vs = kc[:32].clone(), vc[:32].clone()
+    rand = randn(g, 32, nkv, 16, D, dtype=torch.bfloat16)
+    kc[-32:], vc[-32:], ks[:], vs[:] = rand, rand.flip(0), rand, rand.flip(0)
+    ctx = torch.tensor([200, 97], device=cuda, dtype=torch.int32)
+    qkv = randn(g, B, T, (16 + 2 * nkv) * D, dtype=torch.bfloat16)
+    cos, sin = K.rotary_tables(300, D, device=cuda)
+    pos = (ctx[:, None] + torch.arange(T, device=cuda, dtype=torch.int32)).contiguous()
+    outs = []
+    for bt, k, v in ((far, kc, vc), (near, ks, vs)):
+        q = torch.zeros(B, T, 16, D, device=cuda, dtype=torch.bfloat16)
+        K.qk_norm_rotary_append_kv(qkv, pos, cos, sin, bt, ctx, q, k, v, 16, nkv)
+        outs.append((q, K.tree_attention(q, k, v, bt, ctx, None, 0.1), k[-32:].clone(), v[-32:].clone()))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    assert not bool(kc[:-32:1000].any())
+
+
+def test_many_sequences_and_rows(cuda):
+    """More sequences than one launch's lengths hold; every (batch, head) of them equals the call on its own."""
+    g = gen(cuda, 30)
+    B, T, nq, nkv, D = 300, 3, 8, 2, 64
+    ctx = torch.randint(0, 200, (B,), generator=g, device=cuda, dtype=torch.int32)
+    q, kc, vc, bt, _, bits = make_tree(g, cuda, B, T, nq, nkv, D, [200], torch.bfloat16)
+    tl = torch.randint(0, T + 1, (B,), generator=g, device=cuda, dtype=torch.int32)
+    out = torch.full_like(q, 4.0)
+    K.tree_attention(q, kc, vc, bt, ctx, bits, 0.2, tree_lens=tl, out=out)
+    pick = [0, 1, 127, 128, 129, 255, 256, 299]
+    ref, mag, sm = tree_ref(q[pick], kc, vc, bt[pick], ctx[pick], [bits.tolist()[i] for i in pick], 0.2, tl[pick])
+    got = out[pick]
+    check_tree(got, ref, mag, sm, 203, D)
+    dead = torch.arange(T, device=cuda)[None] >= tl[:, None]
+    assert bool((out[dead] == 4).all())
+
+
+def test_gradients_in_a_graph(cuda):
+    """Forward and backward captured through autograd (no eager graph of the leaves alive: torch ties their accumulation
+    nodes to its stream), and as plain calls while one is alive."""
+    g = gen(cuda, 17)
+    q, k = randn(g, 2, 9, 4, 64).requires_grad_(), randn(g, 2, 9, 2, 64).requires_grad_()
+    wq, wk = torch.ones(64, device=cuda).requires_grad_(), torch.ones(64, device=cuda).requires_grad_()
+    cos, sin = K.rotary_tables(9, 64, device=cuda)
+    pos = torch.arange(9, device=cuda, dtype=torch.int32)
+    dq, dk = randn(g, 2, 9, 4, 64), randn(g, 2, 9, 2, 64)
+
+    def step():
+        y = K.qk_norm_rotary(q, k, wq, wk, pos, cos, sin)
+        z = K.rotary(y[0], pos, cos, sin)
+        return torch.autograd.grad((z, y[1]), (q, k, wq, wk), (dq, dk))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        want = step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    alive = K.qk_norm_rotary(q, k, wq, wk, pos, cos, sin)
+    graph2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph2), torch.no_grad():
+        plain = K.qk_norm_rotary_backward(K.rotary(dq, pos, cos, sin, inverse=True), dk, q, k, wq, wk, pos, cos, sin)
+    graph2.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(plain, want)) and alive[0].requires_grad
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals(cuda):
     cos, sin = K.rotary_tables(8, 64, device=cuda)
@@ -753,6 +832,11 @@ def test_refusals(cuda):
     bad("overlaps itself", K.rotary, x, pos, cos, sin, out=torch.zeros(2, 1, 64, device=cuda).expand(2, 3, 64))
     bad("no gradient", K.rotary, x.clone().requires_grad_(), pos, cos, sin, out=x)
     bad("constants", K.rotary, x, pos, cos.clone().requires_grad_(), sin)
+    off = torch.zeros(8 * 32 + 1, device=cuda)[1:].view(8, 32)
+    bad("16-byte aligned", K.rotary, x, pos, off, sin)
+    bad("no gradient|not formed", lambda: torch.autograd.grad(torch.autograd.grad(K.qk_norm_rotary(
+        v := x.clone().requires_grad_(), x, torch.ones(64, device=cuda), torch.ones(64, device=cuda), pos, cos, sin)[0].sum(),
+        v, create_graph=True)[0].sum(), v))
     w = torch.ones(64, device=cuda)
     bad("norm weights", K.qk_norm_rotary, x, x, w, w.half(), pos, cos, sin)
     bad("agree", K.qk_norm_rotary, x, x[:1], w, w, pos, cos, sin)

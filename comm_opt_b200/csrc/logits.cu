@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
   __shared__ float s_val[kThreads];
   __shared__ unsigned long long s_key[kThreads / 32];
   pdl_wait_then_trigger();
-  const int row = blockIdx.x, tid = threadIdx.x;
+  const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const T* in = reinterpret_cast<const T*>(p.logits) + row * p.ld_in;
   T* out = reinterpret_cast<T*>(p.out) + row * p.ld_out;
   // ids up to the row's first 16-byte boundary belong to the first chunk; every chunk then starts on one
@@ -127,9 +127,10 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
   auto mark = [&](int slot) {
     if (slot >= N) atomicOr(&s_mark[(slot - N) >> 5], 1u << ((slot - N) & 31));
   };
-  // biases in tiles of one entry per thread; one warp adds them up 32 at a time, equal ids in their order
+  // biases in tiles of one entry per thread; each warp takes the ids of one residue and adds them up 32 entries at a
+  // time, equal ids in their order
   for (int i0 = 0;;) {
-    const bool mine = bid >= g0 && bid - g0 < n;
+    const bool mine = (unsigned)(bid - g0) < (unsigned)n;
     s_id[tid] = mine ? bid - gs : -1;
     s_val[tid] = bval;
     const int here = biases ? min(kThreads, p.biases - i0) : 0;
@@ -140,19 +141,18 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
       bval = i0 + tid < p.biases ? val[i0 + tid] : 0.f;
     }
     __syncthreads();  // (the first also completes the tables' zeros)
-    if (tid < 32)
-      for (int t0 = 0; t0 < here; t0 += 32) {
-        const int at = s_id[t0 + tid];
-        if (!__any_sync(0xffffffffu, at >= 0)) continue;
-        const unsigned same = __match_any_sync(0xffffffffu, at >= 0 ? at : -1 - tid);
-        if (at >= 0 && (same & ((1u << tid) - 1u)) == 0) {
-          float s = bsum[at];
-          for (unsigned m = same; m; m &= m - 1) s = __fadd_rn(s, s_val[t0 + __ffs(m) - 1]);
-          bsum[at] = s;
-          mark(at);
-        }
-        __syncwarp();
+    for (int t0 = 0; t0 < here; t0 += 32) {
+      const int e = s_id[t0 + lane], at = e >= 0 && e % (kThreads / 32) == warp ? e : -1;
+      if (!__any_sync(0xffffffffu, at >= 0)) continue;
+      const unsigned same = __match_any_sync(0xffffffffu, at >= 0 ? at : -1 - lane);
+      if (at >= 0 && (same & ((1u << lane) - 1u)) == 0) {
+        float s = bsum[at];
+        for (unsigned m = same; m; m &= m - 1) s = __fadd_rn(s, s_val[t0 + __ffs(m) - 1]);
+        bsum[at] = s;
+        mark(at);
       }
+      __syncwarp();
+    }
     if (!more) break;
     __syncthreads();
   }
@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
 #pragma unroll
       for (int k = 0; k < kTile; ++k) {
         const int i = i0 + k * kThreads;
-        if (i < len && t[k] >= g0 && t[k] - g0 < n) {
+        // (one unsigned comparison: ids below 2^31 and negative ones never wrap into the chunk)
+        if (i < len && (unsigned)(t[k] - g0) < (unsigned)n) {
           mark(t[k] - gs);
           if (i < plen)
             atomicOr(cnt + (t[k] - gs), kInPrompt);

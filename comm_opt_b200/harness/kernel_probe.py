@@ -6,6 +6,9 @@ removes the host launch interval), and the command a profiler capture of that ke
     python -m comm_opt_b200.harness.kernel_probe attention --batch 8 --ctx 2048
     python -m comm_opt_b200.harness.kernel_probe decode_ops --batch 8
     python -m comm_opt_b200.harness.kernel_probe allgather --world 8 --rows 16
+    python -m comm_opt_b200.harness.kernel_probe tree_attention --batch 4 --tree 64 --heads 64 --kv-heads 8 --ctx 8192
+    python -m comm_opt_b200.harness.kernel_probe rotary_ops --batch 8 --rows 2048 --heads 32 --kv-heads 8
+    python -m comm_opt_b200.harness.kernel_probe logits --batch 128 --vocab 152064 --ctx 2048
     ncu --set full --clock-control none -k regex:k_oneshot -s 3 -c 1 -o oneshot \
         python -m comm_opt_b200.harness.kernel_probe fused_ar --variant lamport_1s --world 2 --rows 8 --iters 4
 
@@ -139,15 +142,74 @@ def decode_ops(a, dev) -> dict:
     return dict(batch=B, hidden=H, inter=inter, **out)
 
 
+def tree_attention(a, dev) -> dict:
+    """`--tree` drafted tokens per sequence (each hanging from a random earlier one) over `--ctx` cached tokens."""
+    B, T, nq, nkv, D = a.batch, a.tree, a.heads, a.kv_heads, a.head_dim
+    pages = (a.ctx + T + 15) // 16
+    g = torch.Generator(device=dev).manual_seed(0)
+    kc = torch.randn(B * pages, nkv, 16, D, generator=g, device=dev).bfloat16()
+    vc = torch.randn(B * pages, nkv, 16, D, generator=g, device=dev).bfloat16()
+    bt = torch.randperm(B * pages, generator=g, device=dev).to(torch.int32).view(B, pages)
+    q = torch.randn(B, T, nq, D, generator=g, device=dev).bfloat16()
+    parents = (torch.rand(B, T, generator=g, device=dev) * torch.arange(T, device=dev)).long()
+    parents[:, 0] = -1
+    mask, ctx, out = K.tree_mask(parents), torch.full((B,), a.ctx, dtype=torch.int32, device=dev), torch.empty_like(q)
+    r = timed(lambda: K.tree_attention(q, kc, vc, bt, ctx, mask, D ** -0.5, out=out), a.iters)
+    return dict(r, batch=B, tree=T, ctx=a.ctx, heads=nq, kv_heads=nkv, head_dim=D,
+                kv_bytes=4 * B * nkv * (a.ctx + T) * D, tflop=round(4e-12 * B * T * nq * D * (a.ctx + T), 4))
+
+
+def rotary_ops(a, dev) -> dict:
+    """Rotation, QK norm with rotation, its backward, and the append form: `--batch` x `--rows` rows of each."""
+    B, S, nq, nkv, D = a.batch, a.rows, a.heads, a.kv_heads, a.head_dim
+    g = torch.Generator(device=dev).manual_seed(0)
+    qkv = torch.randn(B, S, nq + 2 * nkv, D, generator=g, device=dev).bfloat16()
+    q, k = qkv[:, :, :nq], qkv[:, :, nq:nq + nkv]
+    w = torch.ones(D, device=dev).bfloat16()
+    cos, sin = K.rotary_tables(S, D, 5e5, device=dev)
+    pos = torch.arange(S, dtype=torch.int32, device=dev)
+    pages = (S + 15) // 16
+    kc = torch.zeros(B * pages, nkv, 16, D, device=dev).bfloat16()
+    vc, qo = torch.zeros_like(kc), torch.empty(B, S, nq, D, device=dev).bfloat16()
+    bt = torch.arange(B * pages, dtype=torch.int32, device=dev).view(B, pages)
+    at = torch.zeros(B, dtype=torch.int32, device=dev)
+    dq, dk = torch.randn_like(q), torch.randn_like(k)
+    out = dict(
+        rotary=timed(lambda: K.rotary(q, pos, cos, sin, out=qo), a.iters),
+        qk_norm_rotary=timed(lambda: K.qk_norm_rotary(q, k, w, w, pos, cos, sin), a.iters),
+        backward=timed(lambda: K.qk_norm_rotary_backward(dq, dk, q, k, w, w, pos, cos, sin), a.iters),
+        append=timed(lambda: K.qk_norm_rotary_append_kv(qkv.view(B, S, -1), pos, cos, sin, bt, at, qo, kc, vc, nq, nkv,
+                                                        q_weight=w, k_weight=w), a.iters))
+    return dict(batch=B, rows=S, heads=nq, kv_heads=nkv, head_dim=D, **out)
+
+
+def logits(a, dev) -> dict:
+    """Penalties from histories of `--ctx` tokens, 64 biases and grammar masks on `--batch` rows of `--vocab` logits."""
+    B, V, L = a.batch, a.vocab, a.ctx
+    g = torch.Generator(device=dev).manual_seed(0)
+    x = torch.randn(B, V, generator=g, device=dev)
+    tok = torch.randint(0, V, (B, L), generator=g, device=dev, dtype=torch.int32)
+    one = torch.ones(B, device=dev)
+    ids, bias = torch.randint(0, V, (B, 64), generator=g, device=dev, dtype=torch.int32), torch.randn(B, 64, device=dev)
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (B, (V + 31) // 32), generator=g, device=dev).to(torch.int32)
+    out, keys = torch.empty_like(x), torch.zeros(B, dtype=torch.int64, device=dev)
+    pen = dict(tokens=tok, repetition=1.1 * one, frequency=0.1 * one, presence=0.1 * one, out=out)
+    full = dict(pen, bias_ids=ids, bias=bias, allowed=allowed)
+    return dict(batch=B, vocab=V, history=L, copy=timed(lambda: K.penalize_logits(x, out=out), a.iters),
+                penalties=timed(lambda: K.penalize_logits(x, **pen), a.iters),
+                everything=timed(lambda: K.penalize_logits(x, keys=keys, **full), a.iters))
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("kernel", choices=["fused_ar", "allgather", "attention", "decode_ops"])
+    ap.add_argument("kernel", choices=["fused_ar", "allgather", "attention", "decode_ops", "tree_attention", "rotary_ops", "logits"])
     ap.add_argument("--variant", default="lamport_1s")
     ap.add_argument("--world", type=int, default=2)
     ap.add_argument("--rows", type=int, default=8)
     ap.add_argument("--hidden", type=int, default=8192)
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--ctx", type=int, default=2048)
+    ap.add_argument("--tree", type=int, default=16, help="tree_attention: drafted tokens per sequence")
     ap.add_argument("--heads", type=int, default=8)
     ap.add_argument("--kv-heads", type=int, default=1)
     ap.add_argument("--inter", type=int, default=3584)
@@ -167,7 +229,8 @@ def main():
     if a.attn_stages:
         K.set_attn_stages(a.attn_stages)
     r = {"fused_ar": fused_ar, "allgather": allgather, "attention": attention,
-         "decode_ops": decode_ops}[a.kernel](a, dev)
+         "decode_ops": decode_ops, "tree_attention": tree_attention, "rotary_ops": rotary_ops,
+         "logits": logits}[a.kernel](a, dev)
     print(json.dumps(dict(kernel=a.kernel, **r)))
 
 

@@ -19,11 +19,12 @@
 // L2. A (sequence, head) cut between shares leaves unnormalised partials (at most two per CTA) that a second kernel,
 // launched early, joins in the shares' order.
 //
-// Bounds, measured on one B200 at 4 x 64 drafted tokens over 32k, 64 / 8 heads of 128 (0.55 GB, 275 GFLOP): 287 us, 0.96
+// Bounds, measured on one B200 at 4 x 64 drafted tokens over 32k, 64 / 8 heads of 128 (0.55 GB, 275 GFLOP): 276 us, 1.00
 // PFLOP/s. Without the softmax the same walk takes 222 us, of which Q K^T 97 us: M = 128, N = 64 from shared memory reads
 // 6 KB per 32 cycles of arithmetic and the memory gives 128 bytes a cycle, but 128 columns do not fit beside O twice.
 // Exponentials on the FMA pipe (a degree-5 polynomial for 2 to 4 of 8), 16 softmax warps of 16 rows each (16x256b TMEM
-// accesses) and 128-column steps were all measured and no faster (288 - 303, 306, 305 us).
+// accesses) and 128-column steps were all measured and no faster (288 - 303, 306, 305 us against 290 then); the two row
+// tiles taking turns at the exponential unit took it from 290 to 276.
 // Small: 8 drafted tokens over 1k, 32 / 8 heads: 10.8 us, latencies (lengths, page indices and first pages 3.2, one tile
 // 1.5, output 1, the join 3). 8 x 16 over up to 2k, 64 / 8 heads (38 MB): 21.5 us.
 //
@@ -45,6 +46,7 @@ using namespace sm100;
 
 constexpr int kPage = 16, kTile = 128, kTilePages = kTile / kPage;
 constexpr int kMaxBatch = 128;  // sequences of one launch (their lengths and tile counts live in shared memory)
+constexpr int kBarBytes = 320;  // barriers and flags of a CTA
 constexpr int kPieceCost = 2;   // of starting and ending a piece of a (sequence, KV head), in tiles
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint64_t kTimeout = 1000000000ull;  // of every wait, ns
@@ -222,9 +224,10 @@ struct Geo {
   static constexpr int HALF_BYTES = kTile * 128;          // 64 columns of a tile
   static constexpr int TILE_BYTES = kTile * D * 2;        // Q, K or V tile
   static constexpr int KS = 3, VS = NT == 2 ? 2 : 3;      // ring stages (227 KB per CTA at D = 128)
-  static constexpr int WARPS = 4 * NT + 4;                // 4 softmax warps per row tile, 2 loading, 1 issuing MMAs, 1 idle
+  // 4 softmax warps per row tile, 2 loading, 1 issuing MMAs, 1 idle (with 11 warps the compiler spills)
+  static constexpr int WARPS = 4 * NT + 4;
   static constexpr int THREADS = WARPS * 32;
-  static constexpr int SMEM = 1024 + NT * TILE_BYTES + (KS + VS) * TILE_BYTES + 256 + (3 * kMaxBatch + 1) * 4;
+  static constexpr int SMEM = 1024 + NT * TILE_BYTES + (KS + VS) * TILE_BYTES + kBarBytes + (3 * kMaxBatch + 1) * 4;
   static constexpr int STEP = 64;                         // tokens of a score buffer: two per row tile fit beside O
   static constexpr int PER = kTile / STEP;                // steps of a tile
   static constexpr uint32_t O0 = 256;                     // TMEM columns: score buffers [tile][2] of STEP, then O of each tile
@@ -350,11 +353,12 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
   uint64_t* p_ready = s_full + 2 * NT;   // [NT][2] and its weights
   uint64_t* o_done = p_ready + 2 * NT;   // [NT] one more P V of a row tile has completed
   uint64_t* q_ready = o_done + NT;       // [NT] query tile staged
-  uint64_t* drain = q_ready + NT;
+  uint64_t* turn = q_ready + NT;         // [NT][4] a warp's turn at the exponential unit
+  uint64_t* drain = turn + 4 * NT;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* s_fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_odd = reinterpret_cast<int*>(tmem_slot + 2);  // a drafted v of this segment is not finite
-  Lens lens(reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(k_full) + 256));
+  Lens lens(reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(k_full) + kBarBytes));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int WK = 4 * NT, WV = WK + 1, WM = WK + 2;
@@ -363,6 +367,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     for (int i = 0; i < C::VS; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 2 * NT; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_ready[i], 4);
     for (int i = 0; i < NT; ++i) mbar_init(&o_done[i], 1), mbar_init(&q_ready[i], 4);
+    for (int i = 0; i < 4 * NT; ++i) mbar_init(&turn[i], 1);
     mbar_init(drain, 1);
     *s_fail = 0;
     *s_odd = 0;
@@ -509,6 +514,11 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_ready[tile]);
     };
+    // The two row tiles' warps of one scheduler take turns at their exponentials. Left alone they fall into step, share the
+    // exponential unit while both need it and leave it idle while neither does.
+    auto my_turn = [&](int n) {
+      return NT == 1 || (tile == 0 && n == 0) || warp_wait(&turn[tile * 4 + wq], (tile ? n : n - 1) & 1, s_fail);
+    };
     int n0 = 0, i0 = 0;
     bool okay = true, have = walk.next(sg);
     if (have) {
@@ -622,6 +632,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
               tmem_st32(obuf + 32 * k, o);
             }
           }
+          okay = my_turn(n);
+          if (!okay) break;
           const float mu = m == -INFINITY ? 0.f : m * c;
           const uint64_t c2 = pair(c, c), mu2 = pair(-mu, -mu);
           uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
@@ -635,6 +647,13 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
             w[x / 32][x % 32] = pack2<T>(a, b);
           }
           l += sum2(add2(sum[0], sum[1]));
+        } else {
+          okay = my_turn(n);
+          if (!okay) break;
+        }
+        if (NT == 2) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&turn[(tile ^ 1) * 4 + wq]);
         }
         if (st > 0) {  // the previous P V has long ended; seeing its phase keeps this warp's parity in step
           okay = warp_wait(&o_done[tile], (n - 1) & 1, s_fail);

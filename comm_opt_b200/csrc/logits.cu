@@ -81,16 +81,18 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
     }
   }
   // bit words of the chunk's ids v0 + 32 w ..: allowed, and touched by the history or a bias
+  const int last_word = (p.vocab_offset + p.vocab - 1) >> 5;  // (ids reach 2^31 - 2: words are compared, not their ids)
   constexpr int kWords = MAXV * N * kThreads / 32, kPer = (kWords + kThreads - 1) / kThreads;
   __shared__ uint32_t s_mask[kWords], s_mark[kWords + 1];  // (one more for the ids before v0)
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int w = tid + i * kThreads, g = p.vocab_offset + v0 + 32 * w;
+    const int w = tid + i * kThreads;
     if (w < kWords) {
       s_mark[w] = 0;
       if (mask && 32 * w < v1 - v0) {
+        const int g = p.vocab_offset + v0 + 32 * w;
         const uint32_t a = __ldg(mask + (g >> 5));
-        const uint32_t b = (g & 31) && ((g >> 5) + 1) * 32 < p.vocab_offset + p.vocab ? __ldg(mask + (g >> 5) + 1) : 0u;
+        const uint32_t b = (g & 31) && (g >> 5) < last_word ? __ldg(mask + (g >> 5) + 1) : 0u;
         s_mask[w] = __funnelshift_r(a, b, g & 31);
       }
     }
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
   // biases in tiles of one entry per thread; each warp takes the ids of one residue and adds them up 32 entries at a
   // time, equal ids in their order
   for (int i0 = 0;;) {
-    const bool mine = (unsigned)(bid - g0) < (unsigned)n;
+    const bool mine = (unsigned)bid - (unsigned)g0 < (unsigned)n;
     s_id[tid] = mine ? bid - gs : -1;
     s_val[tid] = bval;
     const int here = biases ? min(kThreads, p.biases - i0) : 0;
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
       for (int k = 0; k < kTile; ++k) {
         const int i = i0 + k * kThreads;
         // (one unsigned comparison: ids below 2^31 and negative ones never wrap into the chunk)
-        if (i < len && (unsigned)(t[k] - g0) < (unsigned)n) {
+        if (i < len && (unsigned)t[k] - (unsigned)g0 < (unsigned)n) {
           mark(t[k] - gs);
           if (i < plen)
             atomicOr(cnt + (t[k] - gs), kInPrompt);

@@ -581,6 +581,34 @@ def test_penalize_logits(cuda, dtype, B, V, L, nb, off):
         assert torch.equal(pad[:, 1:V + 1], y) and bool((pad[:, 0] == 7).all()) and bool((pad[:, V + 1:] == 7).all())
 
 
+def test_penalize_logits_last_ids(cuda):
+    """Ids up to 2^31 - 2: the mask's last word is the row's last, and ids below zero do not wrap into the shard."""
+    V, words = 101, 1 << 26
+    off = 2 ** 31 - 1 - V
+    g = gen(cuda, 9)
+    x = randn(g, 1, V, dtype=torch.float32)
+    allowed = torch.zeros(1, words, dtype=torch.int32, device=cuda)
+    bits = torch.rand(V, generator=g, device=cuda) < 0.6
+    bits[-2:] = torch.tensor([True, False], device=cuda)
+    for v in bits.nonzero()[:, 0].tolist():
+        one = 1 << ((off + v) % 32)
+        allowed[0, (off + v) // 32] |= one - (1 << 32) if one >> 31 else one
+    tokens = torch.tensor([[off + V - 2, off, off - 1, -1, -2 ** 31, 2 ** 31 - 1, 0]], dtype=torch.int32, device=cuda)
+    pres = torch.ones(1, device=cuda)
+    keys = torch.zeros(1, dtype=torch.int64, device=cuda)
+    y = K.penalize_logits(x, vocab_offset=off, allowed=allowed, tokens=tokens, presence=pres, bias_ids=tokens,
+                          bias=torch.full((1, 7), 0.5, device=cuda), keys=keys)
+    ref = x.clone()
+    ref[0, [0, V - 2]] = ref[0, [0, V - 2]] - 1.0 + 0.5
+    ref[0, ~bits] = float("-inf")
+    assert torch.equal(y, ref)
+    assert torch.equal(keys, K.argmax_local(y, off))
+    # the mask as the last row of a tensor that ends with it, at every alignment of the shard in its words
+    for v0 in range(33):
+        y = K.penalize_logits(x[:, v0:], vocab_offset=off + v0, allowed=allowed)
+        assert torch.equal(y[0], torch.where(bits, x[0], float("-inf"))[v0:])
+
+
 def test_penalize_logits_special_values(cuda):
     x = torch.tensor([[float("inf"), -float("inf"), float("nan"), 0.0, -0.0, torch.finfo(torch.bfloat16).min]], device=cuda).bfloat16()
     t = torch.tensor([[0, 1, 2, 3, 4, 5]], device=cuda, dtype=torch.int32)

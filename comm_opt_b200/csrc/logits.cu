@@ -81,18 +81,17 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
     }
   }
   // bit words of the chunk's ids v0 + 32 w ..: allowed, and touched by the history or a bias
-  const int last_word = (p.vocab_offset + p.vocab - 1) >> 5;  // (ids reach 2^31 - 2: words are compared, not their ids)
   constexpr int kWords = MAXV * N * kThreads / 32, kPer = (kWords + kThreads - 1) / kThreads;
   __shared__ uint32_t s_mask[kWords], s_mark[kWords + 1];  // (one more for the ids before v0)
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int w = tid + i * kThreads;
+    const int g = (int)((unsigned)(p.vocab_offset + v0) + 32u * w);
     if (w < kWords) {
       s_mark[w] = 0;
       if (mask && 32 * w < v1 - v0) {
-        const int g = p.vocab_offset + v0 + 32 * w;
         const uint32_t a = __ldg(mask + (g >> 5));
-        const uint32_t b = (g & 31) && (g >> 5) < last_word ? __ldg(mask + (g >> 5) + 1) : 0u;
+        const uint32_t b = (g & 31) && (g | 31) < p.vocab_offset + p.vocab - 1 ? __ldg(mask + (g >> 5) + 1) : 0u;  // (ids reach 2^31 - 2)
         s_mask[w] = __funnelshift_r(a, b, g & 31);
       }
     }

@@ -457,7 +457,8 @@ Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_
     y = tree_lens.has_value() ? torch::zeros(q.sizes(), q.options()) : torch::empty(q.sizes(), q.options());
   }
   if (q.numel() == 0) return y;
-  const Tensor qc = vec_ok(q) ? q : q.contiguous();
+  // (a copy always: contiguous() would hand back a contiguous q whose start is not on a 16-byte boundary)
+  const Tensor qc = vec_ok(q) ? q : q.clone(at::MemoryFormat::Contiguous);
   p.q = qc.data_ptr();
   p.q_sb = qc.stride(0), p.q_st = qc.stride(1), p.q_sh = qc.stride(2);
   p.out = y.data_ptr();

@@ -376,8 +376,11 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     prefetch_tmap(&args.tv);
   }
   if (warp == WM) tmem_alloc(tmem_slot, 512);
-  pdl_wait_then_trigger();
   tc_fence_before();
+  // The dependents may start once every CTA has triggered, and may want tensor memory too: no thread triggers before its
+  // CTA's allocation is done, or a dependent's CTA could take columns first and wait for this kernel, which waits for them.
+  __syncthreads();
+  pdl_wait_then_trigger();
   lens.fill(p);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;

@@ -22,3 +22,34 @@ def test_tree_attention_of_a_misaligned_contiguous_query(cuda, dtype, off):
     odd = flat[off:off + q.numel()].view_as(q).copy_(q)
     assert odd.is_contiguous() and odd.data_ptr() % 16
     assert torch.equal(K.tree_attention(odd, kc, vc, bt, cl, bits, 0.125), K.tree_attention(q, kc, vc, bt, cl, bits, 0.125))
+
+
+# ---------------------------------------------------------------------------------------------- launch order
+def test_tree_attention_between_gemms_with_programmatic_launch(cuda):
+    """Heads of 64 and at most 8 pages a sequence (one kernel, which leaves room for another on its SM) between GEMMs, which
+    take tensor memory too: the same bits as launched one after another."""
+    from comm_opt_b200.models.gemm import gemm, gemm_error_word
+
+    g = gen(cuda, 3)
+    q, kc, vc, bt, cl, bits = make_tree(g, cuda, 2, 8, 8, 2, 64, [60, 33], torch.bfloat16)
+    w = randn(g, 2048, 512, dtype=torch.bfloat16, std=0.05)
+    w2 = randn(g, 512, 2048, dtype=torch.bfloat16, std=0.05)
+
+    def chain():
+        x = q
+        for _ in range(4):
+            o = K.tree_attention(x, kc, vc, bt, cl, bits, 0.125)
+            h = gemm(o.view(16, 512), w, pdl=K.native().get_pdl(), small_smem=True)
+            x = gemm(h, w2, pdl=K.native().get_pdl(), small_smem=True).view_as(q)
+        return x
+
+    assert bt.shape[1] <= 8
+    want = chain()
+    old = K.set_pdl(True)
+    try:
+        got = [chain() for _ in range(20)]
+        torch.cuda.synchronize()
+    finally:
+        K.set_pdl(old)
+    assert all(torch.equal(x, want) for x in got)
+    assert int(gemm_error_word(cuda)) == 0

@@ -485,6 +485,8 @@ Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_
 Tensor py_penalize_logits(Tensor logits, OptTensor tokens, OptTensor lens, OptTensor prompt_lens, OptTensor repetition,
                           OptTensor frequency, OptTensor presence, OptTensor bias_ids, OptTensor bias, OptTensor allowed,
                           int64_t vocab_offset, OptTensor out, OptTensor keys) {
+  // the kernel looks up to 2048 entries ahead in 32-bit indexes, which must not wrap
+  constexpr int64_t kMostEntries = 1ll << 30;
   COB_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be a CUDA tensor [rows, vocab]");
   cob::LogitsParams p;
   p.dtype = code_of(logits, "logits");
@@ -504,8 +506,9 @@ Tensor py_penalize_logits(Tensor logits, OptTensor tokens, OptTensor lens, OptTe
   if (tokens.has_value()) {
     on_device(*tokens, "tokens", logits);
     COB_CHECK(tokens->scalar_type() == torch::kInt && tokens->dim() == 2 && tokens->size(0) == B &&
-                  (tokens->stride(1) == 1 || tokens->size(1) <= 1) && tokens->size(1) < (1ll << 31),
+                  (tokens->stride(1) == 1 || tokens->size(1) <= 1),
               "tokens must be int32 [rows, history], a row's ids contiguous");
+    COB_CHECK(tokens->size(1) <= kMostEntries, "tokens hold at most 2^30 ids a row");
     p.tokens = tokens->data_ptr<int32_t>();
     p.ld_tokens = tokens->stride(0);
     p.history = (int)tokens->size(1);
@@ -525,8 +528,9 @@ Tensor py_penalize_logits(Tensor logits, OptTensor tokens, OptTensor lens, OptTe
   if (bias.has_value()) {
     dense(*bias_ids, "bias_ids", torch::kInt, logits);
     dense(*bias, "bias", torch::kFloat, logits);
-    COB_CHECK(bias->dim() == 2 && bias->size(0) == B && bias->sizes() == bias_ids->sizes() && bias->size(1) < (1ll << 31),
+    COB_CHECK(bias->dim() == 2 && bias->size(0) == B && bias->sizes() == bias_ids->sizes(),
               "bias_ids (int32) and bias (float32) must be [rows, entries]");
+    COB_CHECK(bias->size(1) <= kMostEntries, "a row has at most 2^30 biases");
     p.bias_ids = bias_ids->data_ptr<int32_t>();
     p.bias = bias->data_ptr<float>();
     p.biases = (int)bias->size(1);

@@ -47,9 +47,9 @@ def penalize_logits(logits, *, tokens=None, lens=None, prompt_lens=None, repetit
 
     tokens int32 [rows, history]: the first lens[row] (default all) count, of them the first prompt_lens[row] (default
     none) are the prompt's. repetition, frequency, presence: fp32 [rows] each, None for none. bias_ids int32 and bias fp32
-    [rows, entries]. allowed int32 [rows, words], bit i % 32 of word i / 32 for id i. All ids are global: logits column
-    v is id vocab_offset + v of a vocabulary shard; ids elsewhere (or negative: padding) are skipped. Computed in fp32,
-    rounded once. `out` may be the logits themselves. With `keys` (int64 [rows], zero before use) the stored values'
-    greedy keys are folded in as `argmax_local` does, for `argmax_combine`."""
+    [rows, entries]; at most 2^30 ids and entries a row. allowed int32 [rows, words], bit i % 32 of word i / 32 for id i.
+    All ids are global: logits column v is id vocab_offset + v of a vocabulary shard; ids elsewhere (or negative: padding)
+    are skipped. Computed in fp32, rounded once. `out` may be the logits themselves. With `keys` (int64 [rows], zero
+    before use) the stored values' greedy keys are folded in as `argmax_local` does, for `argmax_combine`."""
     return native().penalize_logits(logits, tokens, lens, prompt_lens, repetition, frequency, presence, bias_ids, bias,
                                     allowed, int(vocab_offset), out, keys)

@@ -53,3 +53,21 @@ def test_tree_attention_between_gemms_with_programmatic_launch(cuda):
         K.set_pdl(old)
     assert all(torch.equal(x, want) for x in got)
     assert int(gemm_error_word(cuda)) == 0
+
+
+# --------------------------------------------------------------------------------------------------- lengths
+def test_histories_and_biases_past_the_kernel_s_indexes_are_refused(cuda):
+    """The kernel steps ahead in 32-bit indexes: rows close to 2^31 entries would wrap and read out of range."""
+    x, one = torch.zeros(1, 64, device=cuda), torch.ones(1, device=cuda)
+    many = torch.empty(1, 2 ** 30 + 1, dtype=torch.int32, device=cuda)
+    with pytest.raises(RuntimeError, match="at most 2\\^30 ids"):
+        K.penalize_logits(x, tokens=many, presence=one)
+    with pytest.raises(RuntimeError, match="at most 2\\^30 biases"):
+        K.penalize_logits(x, bias_ids=many, bias=many.view(torch.float32))
+    # (the longest history that is taken: it ends, and counts what it holds)
+    many = many[:, :2 ** 30].fill_(-1)
+    many[0, [0, 12345, -1]] = torch.tensor([3, 5, 5], dtype=torch.int32, device=cuda)
+    y = K.penalize_logits(x, tokens=many, frequency=one)
+    want = torch.zeros_like(x)
+    want[0, 3], want[0, 5] = -1, -2
+    assert torch.equal(y, want)

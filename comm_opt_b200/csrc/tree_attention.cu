@@ -585,6 +585,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
             }
           }
           fence_proxy_async();
+          __syncwarp();  // (lanes went their own ways; the TMEM accesses are the whole warp's)
         }
         constexpr int G = C::STEP / 32;
         uint32_t w[G / 2][32];
@@ -657,6 +658,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
         if (NT == 2) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&turn[(tile ^ 1) * 4 + wq]);
+          __syncwarp();
         }
         if (st > 0) {  // the previous P V has long ended; seeing its phase keeps this warp's parity in step
           okay = warp_wait(&o_done[tile], (n - 1) & 1, s_fail);
@@ -692,6 +694,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
 #pragma unroll 1
         for (int k = 0; k < D / 32; ++k) {
           uint32_t o[32];
+          __syncwarp();  // (rows differ in what they add back and store)
           tmem_ld32(obuf + 32 * k, o);
           tmem_landed(o);
           if (odd && live) {  // non-finite components of drafted tokens that this row sees, from this segment's tiles

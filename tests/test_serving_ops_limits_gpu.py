@@ -71,3 +71,26 @@ def test_histories_and_biases_past_the_kernel_s_indexes_are_refused(cuda):
     want = torch.zeros_like(x)
     want[0, 3], want[0, 5] = -1, -2
     assert torch.equal(y, want)
+
+
+# ------------------------------------------------------------------------------------------ lanes that part
+@pytest.mark.parametrize("D,T,nq,dtype", [(64, 41, 3, torch.float16), (128, 41, 3, torch.bfloat16), (128, 30, 9, torch.bfloat16)])
+def test_tree_attention_rows_that_add_back_beside_rows_that_do_not(cuda, D, T, nq, dtype):
+    """Non-finite v of single drafted tokens over a context that is cut between shares: in a warp some rows see them, some
+    do not and some are padding. Rows that do not see them keep their bits, the others get the value."""
+    g = gen(cuda, T + nq)
+    q, kc, vc, bt, cl, bits = make_tree(g, cuda, 2, T, nq, 1, D, [5000, 77], dtype)
+    tl = torch.tensor([T - 2, T], dtype=torch.int32, device=cuda)
+    want = K.tree_attention(q, kc, vc, bt, cl, bits, 0.1, tree_lens=tl)
+    bad = vc.clone()
+    seen = torch.zeros(2, T, D, dtype=torch.bool, device=cuda)
+    for b in range(2):
+        for j, d in ((3, 5), (T - 5, 40), (17, D - 1)):
+            slot = int(cl[b]) + j
+            bad[bt[b, slot // 16].long(), 0, slot % 16, d] = float("inf")
+            seen[b, :, d] |= ((bits[b] >> j) & 1).bool()
+        seen[b, int(tl[b]):] = False
+    got = K.tree_attention(q, kc, bad, bt, cl, bits, 0.1, tree_lens=tl)
+    hit = seen[:, :, None].expand_as(got)
+    assert bool((got[hit] == float("inf")).all()) and bool(hit.any())
+    assert torch.equal(got[~hit], want[~hit])

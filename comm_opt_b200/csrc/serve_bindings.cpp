@@ -412,10 +412,11 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
 }
 
 Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor ctx_lens, OptTensor mask,
-                         double scale, OptTensor tree_lens, OptTensor out) {
+                         double scale, OptTensor tree_lens, OptTensor out, int64_t timeout_ns) {
   COB_CHECK(q.is_cuda() && q.dim() == 4, "q must be a CUDA tensor [batch, tree, nq, head_dim]");
   const int dtype = code_of(q, "q");
   COB_CHECK(dtype != cob::kF32, "q and the caches must be float16 or bfloat16");
+  COB_CHECK(timeout_ns >= 0, "timeout_ms must not be negative");
   cob::TreeAttnParams p;
   const int64_t B = q.size(0), T = q.size(1), nq = q.size(2), D = q.size(3);
   COB_CHECK(D == 64 || D == 128, "head_dim must be 64 or 128, got ", D);
@@ -475,11 +476,20 @@ Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_
   p.max_blocks = (int)block_tables.size(1);
   p.num_blocks = (int)k_cache.size(0);
   p.scale = (float)scale;
+  p.timeout_ns = (unsigned long long)timeout_ns;
   p.dtype = dtype;
   // partials of rows cut between CTAs: memory of this call (or of the graph that captures it)
   Tensor scratch = torch::empty({(int64_t)cob::tree_attention_scratch_bytes(p)}, q.options().dtype(torch::kByte).requires_grad(false));
   ok(cob::tree_attention(p, scratch.data_ptr(), cur()), "tree_attention");
   return y;
+}
+
+// the device's word, as a tensor over it
+Tensor py_tree_attention_error_word(int64_t device) {
+  const c10::cuda::CUDAGuard g((c10::DeviceIndex)device);
+  int* word = nullptr;
+  ok(cob::tree_attention_error_word(&word), "tree_attention_error_word");
+  return torch::from_blob(word, {1}, torch::TensorOptions().dtype(torch::kInt).device(torch::kCUDA, (c10::DeviceIndex)device));
 }
 
 Tensor py_penalize_logits(Tensor logits, OptTensor tokens, OptTensor lens, OptTensor prompt_lens, OptTensor repetition,
@@ -583,5 +593,6 @@ void register_serve(pybind11::module& m) {
   m.def("qk_norm_rotary_backward", &py_qk_norm_rotary_backward);
   m.def("qk_norm_rotary_append", &py_qk_norm_rotary_append);
   m.def("tree_attention", &py_tree_attention);
+  m.def("tree_attention_error_word", &py_tree_attention_error_word);
   m.def("penalize_logits", &py_penalize_logits);
 }

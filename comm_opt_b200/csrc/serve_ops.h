@@ -91,8 +91,12 @@ struct TreeAttnParams {
   long long mask_sb = 0;
   int batch = 0, tree = 0, nq = 0, nkv = 0, head_dim = 0, max_blocks = 0, num_blocks = 0;
   float scale = 1.f;
+  unsigned long long timeout_ns = 1000000000ull;  // of every wait inside the kernel; 0: gives up before its first wait
   int dtype = 0;
 };
+// Where a wait runs out, the rows that were still owed become NaN and the current device's word (its address in *word)
+// is set to 1 until the host clears it.
+cudaError_t tree_attention_error_word(int** word);
 // `scratch`: tree_attention_scratch_bytes(p) bytes, 16-byte aligned, of this call alone; any content.
 size_t tree_attention_scratch_bytes(const TreeAttnParams& p);
 cudaError_t tree_attention(const TreeAttnParams& p, void* scratch, cudaStream_t s);

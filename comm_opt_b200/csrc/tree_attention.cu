@@ -49,7 +49,8 @@ constexpr int kMaxBatch = 128;  // sequences of one launch (their lengths and ti
 constexpr int kBarBytes = 320;  // barriers and flags of a CTA
 constexpr int kPieceCost = 2;   // of starting and ending a piece of a (sequence, KV head), in tiles
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint64_t kTimeout = 1000000000ull;  // of every wait, ns
+constexpr uint64_t kDrain = 1000000000ull;  // most that a CTA waits for its own copies and MMAs before it ends, ns
+__device__ int g_gave_up;                   // per device: set where a wait ran out (kept until the host clears it)
 
 // ----------------------------------------------------------------------------- TMEM accesses of this kernel
 // 32 lanes x 32 columns, asynchronous: the registers are valid after tmem_landed()
@@ -201,14 +202,14 @@ __device__ __forceinline__ void quad_transpose(uint4 (&v)[4], int lane) {
 // Bounded wait of a whole warp, one verdict for all lanes (and reconverged: the TMEM accesses that follow need it). The
 // timer and the failure flag are only looked at every 64 tries. Every waiter of a barrier sees every phase of it in turn,
 // so the parity is never ambiguous.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* fail) {
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* fail, uint64_t limit) {
   uint64_t t0 = 0;
   for (uint32_t tries = 1;; ++tries) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     if ((tries & 63u) == 0) {
       const uint64_t t = globaltimer();
       if (t0 == 0) t0 = t;
-      if (__any_sync(0xffffffffu, t - t0 > kTimeout || *fail != 0)) {
+      if (__any_sync(0xffffffffu, t - t0 > limit || *fail != 0)) {
         *fail = 1;
         return false;
       }
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     for (int i = 0; i < NT; ++i) mbar_init(&o_done[i], 1), mbar_init(&q_ready[i], 4);
     for (int i = 0; i < 4 * NT; ++i) mbar_init(&turn[i], 1);
     mbar_init(drain, 1);
-    *s_fail = 0;
+    *s_fail = p.timeout_ns == 0;
     *s_odd = 0;
     fence_barrier_init();
     prefetch_tmap(&args.tk);
@@ -400,7 +401,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     const int stages = is_k ? C::KS : C::VS;
     const int page = lane / C::HALVES, half = lane % C::HALVES;
     int st = 0, ph = 0, issued = 0;
-    bool okay = true;
+    bool okay = p.timeout_ns != 0;
     while (okay && walk.next(sg)) {
       const SeqLen sl = lens.at(p, sg.b);
       const int pages = (sl.len + kPage - 1) / kPage;
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
       int blk = entry(sg.t0);
       for (int t = sg.t0; t < sg.t1; ++t) {
         const int nxt = t + 1 < sg.t1 ? entry(t + 1) : -1;
-        okay = warp_wait(&empty[st], ph ^ 1, s_fail);
+        okay = warp_wait(&empty[st], ph ^ 1, s_fail, p.timeout_ns);
         if (!okay) break;
         const int np = min(kTilePages, pages - t * kTilePages);
         if (lane == 0) mbar_arrive_expect_tx(&full[st], np * C::HALVES * 2048);
@@ -427,8 +428,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
         if (++st == stages) st = 0, ph ^= 1;
       }
     }
-    if (!okay)  // copies in flight must land before the CTA's memory is given back
-      for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(&full[i % stages], (i / stages) & 1, kTimeout);
+    // copies in flight must land before the CTA's memory is given back: those who wait for them may have given up
+    for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(&full[i % stages], (i / stages) & 1, kDrain);
   } else if (warp == WM) {
     // ------------------------------------------------ MMAs: step s of row tile q is S[q][s & 1] = Q K^T, O[q] += P V
     const uint32_t leader = elect_one();
@@ -437,14 +438,14 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     const uint32_t q_desc = desc_low(smem_addr(sQ), 16), k_desc = desc_low(smem_addr(sK), 16);
     const uint32_t v_desc = desc_low(smem_addr(sV), C::HALF_BYTES);
     int n0 = 0, i0 = 0, seg = 0;  // steps, KV tiles and segments before this segment
-    bool okay = true;
+    bool okay = p.timeout_ns != 0;
     while (okay && walk.next(sg)) {
-      for (int q = 0; q < NT && okay; ++q) okay = warp_wait(&q_ready[q], seg & 1, s_fail);
+      for (int q = 0; q < NT && okay; ++q) okay = warp_wait(&q_ready[q], seg & 1, s_fail, p.timeout_ns);
       const int steps = steps_of<C::STEP>(sg, lens.at(p, sg.b).len);
       auto qk = [&](int s, int q) {
         const int i = i0 + s / C::PER, st = i % C::KS, n = n0 + s;
         if (q == 0 && s % C::PER == 0) {
-          if (!warp_wait(&k_full[st], (i / C::KS) & 1, s_fail)) return false;
+          if (!warp_wait(&k_full[st], (i / C::KS) & 1, s_fail, p.timeout_ns)) return false;
           tc_fence_after();
         }
         const uint32_t a = q_desc + q * (C::TILE_BYTES >> 4);
@@ -465,8 +466,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
         const uint32_t b = v_desc + (st * C::TILE_BYTES + s % C::PER * (C::STEP * 128) >> 4);
 #pragma unroll
         for (int q = 0; q < NT; ++q) {
-          okay = okay && warp_wait(&p_ready[2 * q + (n & 1)], (n >> 1) & 1, s_fail);
-          if (q == 0 && s % C::PER == 0) okay = okay && warp_wait(&v_full[st], (i / C::VS) & 1, s_fail);
+          okay = okay && warp_wait(&p_ready[2 * q + (n & 1)], (n >> 1) & 1, s_fail, p.timeout_ns);
+          if (q == 0 && s % C::PER == 0) okay = okay && warp_wait(&v_full[st], (i / C::VS) & 1, s_fail, p.timeout_ns);
           if (!okay) break;
           tc_fence_after();
           const uint32_t a = tmem + (2 * q + (n & 1)) * C::STEP;
@@ -482,11 +483,9 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
       i0 += sg.t1 - sg.t0;
       ++seg;
     }
-    if (!okay) {  // MMAs in flight must end before their memory is given back
-      *s_fail = 1;
-      commit(drain, leader);
-      mbar_wait(drain, 0, kTimeout);
-    }
+    // MMAs in flight must end before their memory is given back: those who wait for them may have given up
+    commit(drain, leader);
+    mbar_wait(drain, 0, kDrain);
     __syncwarp();
   } else if (warp < WK) {
     // ------------------------------------------------ softmax and epilogue: warpgroup `tile`, thread = row
@@ -520,10 +519,10 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     // The two row tiles' warps of one scheduler take turns at their exponentials. Left alone they fall into step, share the
     // exponential unit while both need it and leave it idle while neither does.
     auto my_turn = [&](int n) {
-      return NT == 1 || (tile == 0 && n == 0) || warp_wait(&turn[tile * 4 + wq], (tile ? n : n - 1) & 1, s_fail);
+      return NT == 1 || (tile == 0 && n == 0) || warp_wait(&turn[tile * 4 + wq], (tile ? n : n - 1) & 1, s_fail, p.timeout_ns);
     };
     int n0 = 0, i0 = 0;
-    bool okay = true, have = walk.next(sg);
+    bool okay = p.timeout_ns != 0, have = walk.next(sg);
     if (have) {
       stage_q(sg);
       q_staged();
@@ -546,7 +545,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
         const int n = n0 + st, i = i0 + st / C::PER, s0 = cur.t0 * kTile + st * C::STEP;
         const uint32_t sbuf = tmem + lanes + (2 * tile + (n & 1)) * C::STEP;
         const bool tail = s0 + C::STEP > sl.ctx;
-        okay = warp_wait(&s_full[2 * tile + (n & 1)], (n >> 1) & 1, s_fail);
+        okay = warp_wait(&s_full[2 * tile + (n & 1)], (n >> 1) & 1, s_fail, p.timeout_ns);
         if (!okay) break;
         tc_fence_after();
         if (st + 1 == steps) {  // every Q K^T of this piece has completed: the next piece's queries may be staged
@@ -559,7 +558,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
           constexpr int CELLS = C::HALVES * 8 * C::STEP / 128;
           const int vs = i % C::VS, at = threadIdx.x % C::STEP, sr = st % C::PER * C::STEP + at, slot = s0 + at;
           const int part = threadIdx.x / C::STEP;
-          okay = warp_wait(&v_full[vs], (i / C::VS) & 1, s_fail);
+          okay = warp_wait(&v_full[vs], (i / C::VS) & 1, s_fail, p.timeout_ns);
           if (!okay) break;
           if (slot >= sl.ctx) {
             uint8_t* vr = sV + vs * C::TILE_BYTES + sr * 128;
@@ -623,7 +622,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
           if (rise) m = mn;  // (by row: no row's result depends on another's)
           l *= f;
           if (st > 0 && __any_sync(0xffffffffu, rise)) {  // rescale rows of O, which the previous P V has finished
-            okay = warp_wait(&o_done[tile], (n - 1) & 1, s_fail);
+            okay = warp_wait(&o_done[tile], (n - 1) & 1, s_fail, p.timeout_ns);
             if (!okay) break;
             tc_fence_after();
 #pragma unroll 1
@@ -661,7 +660,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
           __syncwarp();
         }
         if (st > 0) {  // the previous P V has long ended; seeing its phase keeps this warp's parity in step
-          okay = warp_wait(&o_done[tile], (n - 1) & 1, s_fail);
+          okay = warp_wait(&o_done[tile], (n - 1) & 1, s_fail, p.timeout_ns);
           if (!okay) break;
         }
         if (warp_live) {
@@ -676,7 +675,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
       if (!okay) break;
       if (have) q_staged();
       const int tiles = cur.t1 - cur.t0;
-      okay = warp_wait(&o_done[tile], (n0 + steps - 1) & 1, s_fail);
+      okay = warp_wait(&o_done[tile], (n0 + steps - 1) & 1, s_fail, p.timeout_ns);
       if (!okay) break;
       tc_fence_after();
       n0 += steps;
@@ -740,6 +739,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     }
     if (!okay) {
       // a wait gave up: what this CTA still owed reads as NaN
+      asm volatile("cp.async.wait_all;" ::: "memory");
       const float nan = __uint_as_float(0x7fc00000u);
       Walk again{lens.cum, p.batch, p.nkv, beg, beg, end};
       while (again.next(sg)) {
@@ -756,6 +756,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     tc_fence_before();
   }
   __syncthreads();
+  if (threadIdx.x == 0 && *s_fail) atomicOr(&g_gave_up, 1);
   if (warp == WM) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -886,6 +887,8 @@ cudaError_t launch(TreeArgs a, const Plan& pl, cudaStream_t s) {
 }
 
 }  // namespace
+
+cudaError_t tree_attention_error_word(int** word) { return cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_gave_up); }
 
 size_t tree_attention_scratch_bytes(const TreeAttnParams& p) {
   return part_floats(p, plan_of(p)) * sizeof(float);

@@ -6,7 +6,7 @@ import torch
 from .._ext import native
 from .rotary import (qk_norm_rotary, qk_norm_rotary_append_kv, qk_norm_rotary_backward, rotary,  # noqa: F401
                      rotary_tables)
-from .serving import penalize_logits, tree_attention, tree_mask  # noqa: F401
+from .serving import penalize_logits, tree_attention, tree_attention_error_word, tree_mask  # noqa: F401
 
 
 def rmsnorm(x: torch.Tensor, gamma: torch.Tensor, eps: float, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -23,7 +23,14 @@ def tree_mask(parents: torch.Tensor) -> torch.Tensor:
     return bits[..., :T].contiguous()
 
 
-def tree_attention(q, k_cache, v_cache, block_tables, ctx_lens, tree_mask, scale: float, *, tree_lens=None, out=None):
+def tree_attention_error_word(device) -> torch.Tensor:
+    """Per-device int32 that `tree_attention` sets when one of its bounded waits runs out (zero it to go on)."""
+    dev = torch.device(device)
+    return native().tree_attention_error_word(dev.index if dev.index is not None else torch.cuda.current_device())
+
+
+def tree_attention(q, k_cache, v_cache, block_tables, ctx_lens, tree_mask, scale: float, *, tree_lens=None, out=None,
+                   timeout_ms: float = 1000.0):
     """Grouped-query attention of drafted tokens over a paged cache that already holds their k and v.
 
     q [batch, tree, nq, D] (fp16 / bf16, D 64 or 128, any strides, tree <= 64); caches [num_blocks, nkv, 16, D];
@@ -32,8 +39,11 @@ def tree_attention(q, k_cache, v_cache, block_tables, ctx_lens, tree_mask, scale
     tree] or [tree], see `tree_mask`; None: a chain, token t sees 0..t). A row that sees nothing gives zeros; whatever a
     slot that a row does not see holds, infinities and NaN included, does not reach it. With tree_lens (int32 [batch]) rows t >=
     tree_lens[b] are padding: nothing sees them and `out` keeps what it held there (zeros without `out`). Slots past
-    the block table are not seen; a page index outside the cache reads as zeros."""
-    return native().tree_attention(q, k_cache, v_cache, block_tables, ctx_lens, tree_mask, float(scale), tree_lens, out)
+    the block table are not seen; a page index outside the cache reads as zeros. Every wait inside the kernel is bounded by
+    `timeout_ms` (0: it gives up before the first): where one runs out, rows become NaN and `tree_attention_error_word` is
+    set."""
+    return native().tree_attention(q, k_cache, v_cache, block_tables, ctx_lens, tree_mask, float(scale), tree_lens, out,
+                                   int(timeout_ms * 1e6))
 
 
 def penalize_logits(logits, *, tokens=None, lens=None, prompt_lens=None, repetition=None, frequency=None, presence=None,

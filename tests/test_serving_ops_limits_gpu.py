@@ -94,3 +94,26 @@ def test_tree_attention_rows_that_add_back_beside_rows_that_do_not(cuda, D, T, n
     hit = seen[:, :, None].expand_as(got)
     assert bool((got[hit] == float("inf")).all()) and bool(hit.any())
     assert torch.equal(got[~hit], want[~hit])
+
+
+# ----------------------------------------------------------------------------------------- waits that run out
+def test_tree_attention_wait_that_gives_up_is_reported(cuda):
+    """With no time to wait every row that the call owes reads as NaN, padding keeps its value, and the device's word is set
+    until it is cleared; the next call is a normal one. (Whole pieces and pieces cut between shares, one and two row tiles.)"""
+    g = gen(cuda, 12)
+    word = K.tree_attention_error_word(cuda)
+    assert word.shape == (1,) and word.dtype == torch.int32 and int(word) == 0
+    for B, T, nq, nkv, D, ctx in ((2, 5, 8, 2, 64, [40, 3]), (2, 40, 8, 1, 128, [3000, 9]), (3, 9, 2, 1, 128, [0, 700, 64])):
+        q, kc, vc, bt, cl, bits = make_tree(g, cuda, B, T, nq, nkv, D, ctx, torch.bfloat16)
+        tl = torch.full((B,), T, dtype=torch.int32, device=cuda)
+        tl[-1] = 2
+        want = K.tree_attention(q, kc, vc, bt, cl, bits, 0.1, tree_lens=tl)
+        out = torch.full_like(q, 6.0)
+        K.tree_attention(q, kc, vc, bt, cl, bits, 0.1, tree_lens=tl, out=out, timeout_ms=0)
+        live = torch.arange(T, device=cuda)[None] < tl[:, None]
+        assert bool(out[live].isnan().all()) and bool((out[~live] == 6).all())
+        assert int(K.tree_attention_error_word(cuda)) == 1
+        word.zero_()
+        assert torch.equal(K.tree_attention(q, kc, vc, bt, cl, bits, 0.1, tree_lens=tl), want) and int(word) == 0
+    with pytest.raises(RuntimeError, match="timeout_ms"):
+        K.tree_attention(q, kc, vc, bt, cl, bits, 0.1, timeout_ms=-1)

@@ -4,6 +4,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <tuple>
 #include <utility>
 #include <vector>
@@ -42,9 +43,23 @@ void dense(const Tensor& t, const char* n, torch::ScalarType ty, const Tensor& r
   COB_CHECK(t.is_contiguous(), n, " must be contiguous");
 }
 
-bool same_storage(const Tensor& a, const Tensor& b) {
-  return a.numel() > 0 && b.numel() > 0 && a.storage().data() == b.storage().data();
+// first byte and the one past the last that a tensor's elements reach
+std::pair<uintptr_t, uintptr_t> bytes_of(const Tensor& t) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr());
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return {a, a + (last + 1) * t.element_size()};
 }
+bool overlap(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto x = bytes_of(a), y = bytes_of(b);
+  return x.first < y.second && y.first < x.second;
+}
+// what a call writes lies apart from all of the others
+void apart(const Tensor& t, const char* n, std::initializer_list<const Tensor*> others) {
+  for (const Tensor* o : others) COB_CHECK(!o || !overlap(t, *o), n, " must lie in memory of its own: it overlaps another operand");
+}
+const Tensor* given(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }
 
 // an output that writes every element once: no dimension folded onto itself
 void writable(const Tensor& t, const char* n) {
@@ -137,9 +152,8 @@ Tensor py_rotary(Tensor x, Tensor positions, Tensor cos_t, Tensor sin_t, bool in
               "out must have x's shape and type, components contiguous");
     writable(y, "out");
     const bool in_place = y.data_ptr() == x.data_ptr() && y.strides() == x.strides();
-    COB_CHECK(in_place || !same_storage(x, y), "out must be x itself or lie in memory of its own");
-    COB_CHECK(!same_storage(y, positions) && !same_storage(y, cos_t) && !same_storage(y, sin_t),
-              "out overlaps an input");
+    COB_CHECK(in_place || !overlap(x, y), "out must be x itself or lie in memory of its own");
+    apart(y, "out", {&positions, &cos_t, &sin_t});
   }
   const c10::cuda::CUDAGuard g(x.device());
   if (!out.has_value()) y = torch::empty(x.sizes(), x.options().requires_grad(false));
@@ -343,9 +357,12 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
   dense(q_out, "q_out", qkv.scalar_type(), qkv);
   COB_CHECK(q_out.numel() == B * S * nq * D, "q_out must hold batch x seq x nq x head_dim elements");
   cache_ok(k_cache, v_cache, block_tables, qkv, nkv, D, B);
-  COB_CHECK(!same_storage(q_out, qkv) && !same_storage(k_cache, qkv) && !same_storage(v_cache, qkv) &&
-                !same_storage(q_out, k_cache) && !same_storage(q_out, v_cache) && k_cache.data_ptr() != v_cache.data_ptr(),
+  COB_CHECK(!overlap(q_out, qkv) && !overlap(k_cache, qkv) && !overlap(v_cache, qkv) && !overlap(q_out, k_cache) &&
+                !overlap(q_out, v_cache) && !overlap(k_cache, v_cache),
             "q_out and the caches must lie in memory of their own");
+  const std::pair<const Tensor*, const char*> written[3] = {{&q_out, "q_out"}, {&k_cache, "k_cache"}, {&v_cache, "v_cache"}};
+  for (const auto& w : written)
+    apart(*w.first, w.second, {&positions, &cos_t, &sin_t, &block_tables, &starts, given(wq), given(wk), given(lens), given(bias)});
   COB_CHECK(wq.has_value() == wk.has_value(), "give both norm weights or neither");
   cob::RotaryParams p;
   Tensor like = qkv;  // type and device of the operands; head_dim components
@@ -451,8 +468,7 @@ Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_
     COB_CHECK(y.sizes() == q.sizes() && y.scalar_type() == q.scalar_type(), "out must have q's shape and type");
     COB_CHECK(y.numel() == 0 || vec_ok(y), "out's heads must be contiguous and 16-byte aligned");
     writable(y, "out");
-    COB_CHECK(!same_storage(y, q) && !same_storage(y, k_cache) && !same_storage(y, v_cache),
-              "out must lie in memory of its own");
+    apart(y, "out", {&q, &k_cache, &v_cache, &block_tables, &ctx_lens, given(mask), given(tree_lens)});
   } else {
     // rows past tree_lens are not written: give them a value
     y = tree_lens.has_value() ? torch::zeros(q.sizes(), q.options()) : torch::empty(q.sizes(), q.options());
@@ -566,10 +582,17 @@ Tensor py_penalize_logits(Tensor logits, OptTensor tokens, OptTensor lens, OptTe
     COB_CHECK(y.sizes() == logits.sizes() && y.scalar_type() == logits.scalar_type() && (y.stride(1) == 1 || V == 1),
               "out must have the logits' shape and type, a row's values contiguous");
     writable(y, "out");
-    COB_CHECK((y.data_ptr() == logits.data_ptr() && y.strides() == logits.strides()) || !same_storage(y, logits),
+    COB_CHECK((y.data_ptr() == logits.data_ptr() && y.strides() == logits.strides()) || !overlap(y, logits),
               "out must be the logits themselves or lie in memory of its own");
   } else {
     y = torch::empty(logits.sizes(), logits.options());
+  }
+  const std::initializer_list<const Tensor*> inputs = {given(tokens),   given(lens),     given(prompt_lens), given(repetition), given(frequency),
+                                                       given(presence), given(bias_ids), given(bias),        given(allowed)};
+  if (out.has_value()) apart(y, "out", inputs);
+  if (keys.has_value()) {
+    apart(*keys, "keys", inputs);
+    apart(*keys, "keys", {&logits, &y});
   }
   if (B == 0) return y;
   p.logits = logits.data_ptr();

@@ -1,6 +1,8 @@
 """Calls of the rotary, tree-attention and logits operators at the edges of what they allow: alignment, aliasing, extreme
 values, launch order, autograd's modes, and the kernel forms that only many rows select."""
 
+import math
+
 import pytest
 import torch
 
@@ -117,3 +119,78 @@ def test_tree_attention_wait_that_gives_up_is_reported(cuda):
         assert torch.equal(K.tree_attention(q, kc, vc, bt, cl, bits, 0.1, tree_lens=tl), want) and int(word) == 0
     with pytest.raises(RuntimeError, match="timeout_ms"):
         K.tree_attention(q, kc, vc, bt, cl, bits, 0.1, timeout_ms=-1)
+
+
+# ------------------------------------------------------------------------------------------- shared allocations
+def test_disjoint_parts_of_one_allocation_are_taken(cuda):
+    """Operands and outputs cut from one arena give what operands of their own give."""
+    g = gen(cuda, 6)
+    B, S, nq, nkv, D = 2, 3, 4, 2, 64
+    n = nq + 2 * nkv
+    cos, sin = K.rotary_tables(64, D, device=cuda)
+    pos = torch.arange(S, device=cuda, dtype=torch.int32)
+    sizes = dict(qkv=(B, S, n * D), q=(B, S, nq, D), k=(8, nkv, 16, D), v=(8, nkv, 16, D), o=(B, S, nq, D))
+    arena = randn(g, sum(math.prod(s) for s in sizes.values()), dtype=torch.bfloat16)
+    part, at = {}, 0
+    for name, s in sizes.items():
+        part[name] = arena[at:at + math.prod(s)].view(s)
+        at += math.prod(s)
+    own = {name: t.clone() for name, t in part.items()}
+    bt = torch.arange(8, device=cuda, dtype=torch.int32).view(B, 4)
+    at0 = torch.tensor([5, 30], device=cuda, dtype=torch.int32)
+    for t in (part, own):
+        K.qk_norm_rotary_append_kv(t["qkv"], pos, cos, sin, bt, at0, t["q"], t["k"], t["v"], nq, nkv)
+        K.tree_attention(t["q"], t["k"], t["v"], bt, at0, None, 0.125, out=t["o"])
+        K.rotary(t["q"], pos, cos, sin, out=t["qkv"].view(-1)[:t["q"].numel()].view(t["q"].shape))
+    assert all(torch.equal(part[name], own[name]) for name in sizes)
+    two = randn(g, 2, 4, 100)
+    want = K.penalize_logits(two[0].clone(), allowed=torch.full((4, 4), 5, dtype=torch.int32, device=cuda))
+    assert torch.equal(K.penalize_logits(two[0], allowed=torch.full((4, 4), 5, dtype=torch.int32, device=cuda), out=two[1]), want)
+    assert torch.equal(two[1], want)
+
+
+def test_overlapping_operands_are_refused(cuda):
+    """What a call writes lies apart from everything else it reads or writes, whatever the views' types and starts."""
+    cos, sin = K.rotary_tables(64, 64, device=cuda)
+
+    def bad(fn, *a, **k):
+        with pytest.raises(RuntimeError, match="overlap|memory of"):
+            fn(*a, **k)
+
+    raw = torch.zeros(1 << 16, dtype=torch.uint8, device=cuda)
+
+    def cut(dtype, start, *shape):
+        n = math.prod(shape) * dtype.itemsize
+        return raw[start:start + n].view(dtype).view(shape)
+
+    pos = torch.zeros(2, dtype=torch.int32, device=cuda)
+    x = torch.zeros(2, 3, 64, device=cuda)
+    bad(K.rotary, x, cut(torch.int32, 0, 2), cos, sin, out=cut(torch.float32, 0, 2, 3, 64))
+    c2 = cut(torch.float32, 1024, 4, 32)
+    bad(K.rotary, x, pos, c2, sin[:4].clone(), out=cut(torch.float32, 0, 2, 3, 64))
+    bad(K.rotary, cut(torch.float32, 256, 2, 3, 64), pos, cos, sin, out=cut(torch.float32, 0, 2, 3, 64))
+    # caches that share pages, and an append over what it reads
+    kv = torch.zeros(4, 2, 16, 64, device=cuda).half()
+    qkv = torch.zeros(1, 2, 8 * 64, device=cuda).half()
+    bt, st = torch.zeros(1, 2, dtype=torch.int32, device=cuda), torch.zeros(1, dtype=torch.int32, device=cuda)
+    q = torch.zeros(1, 2, 4, 64, device=cuda).half()
+    ok = dict(positions=pos, cos=cos, sin=sin, block_tables=bt, starts=st, q_out=q, k_cache=kv, v_cache=kv.clone(), nq=4, nkv=2)
+    bad(K.qk_norm_rotary_append_kv, qkv, **{**ok, "k_cache": kv[:3], "v_cache": kv[1:]})
+    bad(K.qk_norm_rotary_append_kv, qkv, **{**ok, "q_out": kv.view(-1)[100:612].view(1, 2, 4, 64)})
+    bad(K.qk_norm_rotary_append_kv, qkv, **{**ok, "q_out": cut(torch.half, 0, 1, 2, 4, 64), "positions": cut(torch.int32, 1016, 2)})
+    bad(K.qk_norm_rotary_append_kv, qkv, **{**ok, "q_out": cut(torch.half, 0, 1, 2, 4, 64), "block_tables": cut(torch.int32, 512, 1, 2)})
+    bad(K.qk_norm_rotary_append_kv, qkv, **{**ok, "q_out": cut(torch.half, 0, 1, 2, 4, 64)}, bias=cut(torch.half, 1000, 512))
+    # tree attention over its own queries' tail, mask and lengths
+    o = cut(torch.half, 0, 1, 2, 4, 64)
+    bad(K.tree_attention, cut(torch.half, 512, 1, 2, 4, 64), kv, kv.clone(), bt, st, None, 0.1, out=o)
+    bad(K.tree_attention, q, kv, kv.clone(), bt, st, cut(torch.int64, 512, 2), 0.1, out=o)
+    bad(K.tree_attention, q, kv, kv.clone(), bt, cut(torch.int32, 64, 1), None, 0.1, out=o)
+    # logits
+    y, L = cut(torch.float32, 0, 2, 64), torch.zeros(2, 64, device=cuda)
+    one = torch.ones(2, device=cuda)
+    bad(K.penalize_logits, L, tokens=cut(torch.int32, 64, 2, 4), presence=one, out=y)
+    bad(K.penalize_logits, L, allowed=cut(torch.int32, 64, 2, 2), out=y)
+    bad(K.penalize_logits, L, keys=cut(torch.int64, 64, 2), out=y)
+    bad(K.penalize_logits, L, tokens=torch.zeros(2, 4, dtype=torch.int32, device=cuda), presence=cut(torch.float32, 64, 2), out=y)
+    bad(K.penalize_logits, y, keys=cut(torch.int64, 64, 2))
+    torch.cuda.synchronize()

@@ -75,6 +75,12 @@ void writable(const Tensor& t, const char* n) {
   }
 }
 
+// a caller's tensor that a kernel writes: autograd must see that a value saved for a backward pass has changed (tensors
+// of inference mode have no version)
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 struct Tables {
   int max_pos, rot;
 };
@@ -170,6 +176,7 @@ Tensor py_rotary(Tensor x, Tensor positions, Tensor cos_t, Tensor sin_t, bool in
   p.inverse = inverse;
   p.dtype = code_of(x, "x");
   ok(cob::rotary_forward(p, cur()), "rotary");
+  if (out.has_value()) written(y);
   return y;
 }
 
@@ -360,8 +367,8 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
   COB_CHECK(!overlap(q_out, qkv) && !overlap(k_cache, qkv) && !overlap(v_cache, qkv) && !overlap(q_out, k_cache) &&
                 !overlap(q_out, v_cache) && !overlap(k_cache, v_cache),
             "q_out and the caches must lie in memory of their own");
-  const std::pair<const Tensor*, const char*> written[3] = {{&q_out, "q_out"}, {&k_cache, "k_cache"}, {&v_cache, "v_cache"}};
-  for (const auto& w : written)
+  const std::pair<const Tensor*, const char*> outs[3] = {{&q_out, "q_out"}, {&k_cache, "k_cache"}, {&v_cache, "v_cache"}};
+  for (const auto& w : outs)
     apart(*w.first, w.second, {&positions, &cos_t, &sin_t, &block_tables, &starts, given(wq), given(wk), given(lens), given(bias)});
   COB_CHECK(wq.has_value() == wk.has_value(), "give both norm weights or neither");
   cob::RotaryParams p;
@@ -426,6 +433,7 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
   p.num_blocks = (int)k_cache.size(0);
   p.dtype = code_of(qkv, "qkv");
   ok(cob::rotary_forward(p, cur()), "qk_norm_rotary_append_kv");
+  for (const auto& w : outs) written(*w.first);
 }
 
 Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor ctx_lens, OptTensor mask,
@@ -497,6 +505,7 @@ Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_
   // partials of rows cut between CTAs: memory of this call (or of the graph that captures it)
   Tensor scratch = torch::empty({(int64_t)cob::tree_attention_scratch_bytes(p)}, q.options().dtype(torch::kByte).requires_grad(false));
   ok(cob::tree_attention(p, scratch.data_ptr(), cur()), "tree_attention");
+  if (out.has_value()) written(y);
   return y;
 }
 
@@ -603,6 +612,8 @@ Tensor py_penalize_logits(Tensor logits, OptTensor tokens, OptTensor lens, OptTe
   p.vocab = (int)V;
   p.vocab_offset = (int)vocab_offset;
   ok(cob::penalize_logits(p, cur()), "penalize_logits");
+  if (out.has_value()) written(y);
+  if (keys.has_value()) written(*keys);
   return y;
 }
 

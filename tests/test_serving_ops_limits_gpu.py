@@ -194,3 +194,49 @@ def test_overlapping_operands_are_refused(cuda):
     bad(K.penalize_logits, L, tokens=torch.zeros(2, 4, dtype=torch.int32, device=cuda), presence=cut(torch.float32, 64, 2), out=y)
     bad(K.penalize_logits, y, keys=cut(torch.int64, 64, 2))
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------------- autograd
+def _calls(dev, dtype=torch.float32):
+    """name -> (call, tensors that it writes in place)."""
+    cos, sin = K.rotary_tables(64, 64, device=dev)
+    pos = torch.arange(2, dtype=torch.int32, device=dev)
+    x, y = torch.randn(2, 3, 64, device=dev), torch.empty(2, 3, 64, device=dev)
+    h = torch.randn(1, 2, 4, 64, device=dev).half()
+    kc, vc = torch.randn(3, 2, 16, 64, device=dev).half(), torch.randn(3, 2, 16, 64, device=dev).half()
+    bt, cl = torch.arange(2, dtype=torch.int32, device=dev).view(1, 2), torch.zeros(1, dtype=torch.int32, device=dev)
+    qkv, o = torch.randn(1, 2, 8 * 64, device=dev).half(), torch.empty_like(h)
+    L, M = torch.randn(2, 64, device=dev), torch.empty(2, 64, device=dev)
+    keys = torch.zeros(2, dtype=torch.int64, device=dev)
+    return dict(
+        rotary_in_place=(lambda: K.rotary(x, pos, cos, sin, out=x), [x]),
+        rotary_out=(lambda: K.rotary(x, pos, cos, sin, out=y), [y]),
+        append=(lambda: K.qk_norm_rotary_append_kv(qkv, pos, cos, sin, bt, cl, o, kc, vc, 4, 2), [o, kc, vc]),
+        tree=(lambda: K.tree_attention(h, kc, vc, bt, cl, None, 0.1, out=o), [o]),
+        logits_in_place=(lambda: K.penalize_logits(L, out=L, keys=keys), [L, keys]),
+        logits_out=(lambda: K.penalize_logits(L, out=M), [M]))
+
+
+def test_outputs_written_in_place_raise_their_version(cuda):
+    for name, (call, written) in _calls(cuda).items():
+        before = [t._version for t in written]
+        call()
+        assert all(t._version > v for t, v in zip(written, before)), name
+    # a value that a backward pass needs, overwritten before it: refused, as for torch's own operators
+    cos, sin = K.rotary_tables(8, 64, device=cuda)
+    pos, w = torch.arange(3, device=cuda, dtype=torch.int32), torch.ones(64, device=cuda)
+    q = torch.randn(3, 2, 64, device=cuda, requires_grad=True)
+    k = torch.randn(3, 1, 64, device=cuda)
+    p = q * 1.0
+    y, _ = K.qk_norm_rotary(p, k, w, w, pos, cos, sin)
+    with torch.no_grad():
+        K.rotary(p, pos, cos, sin, out=p)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    # tensors made in inference mode have no version: written as before, inside and outside of it
+    with torch.inference_mode():
+        for call, _ in _calls(cuda).values():
+            call()
+        late = _calls(cuda)
+    for call, _ in late.values():
+        call()

@@ -81,6 +81,19 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// Derivatives that are not formed must not be lost silently: operands of calls without a backward pass take no gradient
+// (while gradients are recorded), and none of the calls takes a forward-mode tangent.
+void no_tangent(const char* op, std::initializer_list<const Tensor*> operands) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : operands) COB_CHECK(!t || !t->_fw_grad(0).defined(), op, " has no forward-mode derivative");
+}
+void constants(const char* op, std::initializer_list<const Tensor*> operands) {
+  if (torch::GradMode::is_enabled())
+    for (const Tensor* t : operands)
+      COB_CHECK(!t || !t->requires_grad(), op, " forms no gradient: call it under torch.no_grad(), or with detached operands");
+  no_tangent(op, operands);
+}
+
 struct Tables {
   int max_pos, rot;
 };
@@ -147,6 +160,7 @@ void operand_ok(const Tensor& x, const char* n) {
 
 Tensor py_rotary(Tensor x, Tensor positions, Tensor cos_t, Tensor sin_t, bool interleaved, bool inverse, OptTensor out) {
   operand_ok(x, "x");
+  constants("rotary", {&x, given(out)});
   cob::RotaryParams p;
   const Tables t = tables(cos_t, sin_t, x.size(-1), x);
   rows_of(x, positions, p);
@@ -198,6 +212,7 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
 };
 
 Tensor py_rotary_autograd(Tensor x, Tensor positions, Tensor cos_t, Tensor sin_t, bool interleaved, bool inverse) {
+  no_tangent("rotary", {&x});
   return RotaryFn::apply(x, positions, cos_t, sin_t, interleaved, inverse);
 }
 
@@ -226,6 +241,7 @@ void pair_ok(const Tensor& q, const Tensor& k) {
 std::tuple<Tensor, Tensor> py_qk_norm_rotary(Tensor q, Tensor k, Tensor wq, Tensor wk, Tensor positions, Tensor cos_t,
                                              Tensor sin_t, double eps, bool interleaved) {
   pair_ok(q, k);
+  constants("qk_norm_rotary", {&q, &k, &wq, &wk});
   cob::RotaryParams p;
   const Tables t = tables(cos_t, sin_t, q.size(-1), q);
   rows_of(q, positions, p);
@@ -256,6 +272,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> py_qk_norm_rotary_backward(Tensor dq,
                                                                       Tensor cos_t, Tensor sin_t, double eps,
                                                                       bool interleaved) {
   pair_ok(q, k);
+  no_tangent("qk_norm_rotary_backward", {&dq, &dk, &q, &k, &wq, &wk});
   on_device(dq, "dq", q);
   on_device(dk, "dk", q);
   COB_CHECK(dq.sizes() == q.sizes() && dk.sizes() == k.sizes() && dq.scalar_type() == q.scalar_type() &&
@@ -316,6 +333,7 @@ struct QkNormRotaryFn : public torch::autograd::Function<QkNormRotaryFn> {
 
 std::tuple<Tensor, Tensor> py_qk_norm_rotary_autograd(Tensor q, Tensor k, Tensor wq, Tensor wk, Tensor positions,
                                                       Tensor cos_t, Tensor sin_t, double eps, bool interleaved) {
+  no_tangent("qk_norm_rotary", {&q, &k, &wq, &wk});
   auto y = QkNormRotaryFn::apply(q, k, wq, wk, positions, cos_t, sin_t, eps, interleaved);
   return {y[0], y[1]};
 }
@@ -345,6 +363,7 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
                               OptTensor wq, OptTensor wk, double eps, OptTensor lens, OptTensor bias, bool interleaved) {
   COB_CHECK(qkv.is_cuda() && (qkv.dim() == 2 || qkv.dim() == 3), "qkv must be a CUDA tensor [batch, seq, width] or [batch * seq, width]");
   code_of(qkv, "qkv");
+  constants("qk_norm_rotary_append_kv", {&qkv, &q_out, &k_cache, &v_cache, given(wq), given(wk), given(bias)});
   COB_CHECK(nq >= 1 && nkv >= 1, "nq and nkv must be positive");
   on_device(starts, "starts", qkv);
   const int64_t B = starts.numel(), W = qkv.size(-1), n = nq + 2 * nkv;
@@ -441,6 +460,7 @@ Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_
   COB_CHECK(q.is_cuda() && q.dim() == 4, "q must be a CUDA tensor [batch, tree, nq, head_dim]");
   const int dtype = code_of(q, "q");
   COB_CHECK(dtype != cob::kF32, "q and the caches must be float16 or bfloat16");
+  constants("tree_attention", {&q, &k_cache, &v_cache, given(out)});
   COB_CHECK(timeout_ns >= 0, "timeout_ms must not be negative");
   cob::TreeAttnParams p;
   const int64_t B = q.size(0), T = q.size(1), nq = q.size(2), D = q.size(3);
@@ -525,6 +545,7 @@ Tensor py_penalize_logits(Tensor logits, OptTensor tokens, OptTensor lens, OptTe
   COB_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be a CUDA tensor [rows, vocab]");
   cob::LogitsParams p;
   p.dtype = code_of(logits, "logits");
+  constants("penalize_logits", {&logits, given(repetition), given(frequency), given(presence), given(bias), given(out)});
   const int64_t B = logits.size(0), V = logits.size(1);
   COB_CHECK(V >= 1 && V <= (1 << 26) && B < (1ll << 31), "logits must be [rows, vocab] with 1 to 2^26 ids");
   COB_CHECK(logits.stride(1) == 1 || V == 1, "a row's logits must be contiguous");

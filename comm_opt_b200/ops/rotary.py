@@ -70,7 +70,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: tor
     """Rotate x [tokens, heads, D] or [batch, seq, heads, D] (fp32, fp16, bf16; any strides) by its positions
     (int32 [seq] or [batch, seq]) and the tables cos, sin (fp32 [max_pos, rotary_dim / 2], see `rotary_tables`).
 
-    Differentiable in x. ``inverse`` rotates back. ``out`` may be x (in place, no gradient) or other memory. A row whose
+    Differentiable in x (reverse mode). ``inverse`` rotates back. ``out`` may be x (in place, no gradient) or other memory. A row whose
     position lies outside the tables becomes zeros (and has a zero gradient): padded rows carry position -1."""
     if out is None and x.requires_grad and torch.is_grad_enabled():
         return native().rotary_autograd(x, positions, cos, sin, bool(interleaved), bool(inverse))
@@ -84,7 +84,7 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, cos, sin, eps: float = 1
     (shapes, positions and tables as in `rotary`); the norms are over each head's D components, their weights [D] of
     the operands' type or fp32. fp32 inside, one rounding at the end.
 
-    Differentiable in q, k and both weights. `qk_norm_rotary_backward` is the same gradient as a plain call: it can be
+    Differentiable in q, k and both weights (reverse mode, once). `qk_norm_rotary_backward` is the same gradient as a plain call: it can be
     captured in a CUDA graph whatever else is alive, which torch allows for autograd only while no eager graph of the same
     leaves is."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or
@@ -96,7 +96,8 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, cos, sin, eps: float = 1
 def qk_norm_rotary_backward(dq, dk, q, k, q_weight, k_weight, positions, cos, sin, eps: float = 1e-6, *,
                             interleaved: bool = False):
     """Gradients (q, k, q_weight, k_weight) of `qk_norm_rotary` from those of its outputs. The weights' gradients are
-    summed in fp32 in a fixed order (equal inputs give equal bits) and rounded to the weights' type."""
+    summed in fp32 in a fixed order (equal inputs give equal bits) and rounded to the weights' type. The results are
+    constants: what requires a gradient is taken as its value."""
     return native().qk_norm_rotary_backward(dq, dk, q, k, q_weight, k_weight, positions, cos, sin, float(eps),
                                             bool(interleaved))
 
@@ -111,7 +112,7 @@ def qk_norm_rotary_append_kv(qkv, positions, cos, sin, block_tables, starts, q_o
     starts[b] + s (int32 [batch]) and is rotated by positions[b, s] (int32; a drafted token's position is its depth, not
     its slot). q_out [batch, seq, nq, D]; caches [num_blocks, nkv, 16, D] (fp32, fp16, bf16) paged by block_tables
     [batch, max_blocks]. Rows s >= lens[b], and rows whose position lies outside the tables, are left out: q_out and the
-    caches keep what they held. k and v of rows whose slot or page does not exist are dropped."""
+    caches keep what they held. k and v of rows whose slot or page does not exist are dropped. No gradient is formed."""
     native().qk_norm_rotary_append(qkv, positions, cos, sin, block_tables, starts, q_out, k_cache, v_cache, int(nq),
                                    int(nkv), q_weight, k_weight, float(eps), lens, bias, bool(interleaved))
     return q_out

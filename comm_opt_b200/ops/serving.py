@@ -41,7 +41,7 @@ def tree_attention(q, k_cache, v_cache, block_tables, ctx_lens, tree_mask, scale
     tree_lens[b] are padding: nothing sees them and `out` keeps what it held there (zeros without `out`). Slots past
     the block table are not seen; a page index outside the cache reads as zeros. Every wait inside the kernel is bounded by
     `timeout_ms` (0: it gives up before the first): where one runs out, rows become NaN and `tree_attention_error_word` is
-    set."""
+    set. No gradient is formed."""
     return native().tree_attention(q, k_cache, v_cache, block_tables, ctx_lens, tree_mask, float(scale), tree_lens, out,
                                    int(timeout_ms * 1e6))
 
@@ -60,6 +60,7 @@ def penalize_logits(logits, *, tokens=None, lens=None, prompt_lens=None, repetit
     [rows, entries]; at most 2^30 ids and entries a row. allowed int32 [rows, words], bit i % 32 of word i / 32 for id i.
     All ids are global: logits column v is id vocab_offset + v of a vocabulary shard; ids elsewhere (or negative: padding)
     are skipped. Computed in fp32, rounded once. `out` may be the logits themselves. With `keys` (int64 [rows], zero
-    before use) the stored values' greedy keys are folded in as `argmax_local` does, for `argmax_combine`."""
+    before use) the stored values' greedy keys are folded in as `argmax_local` does, for `argmax_combine`. No gradient is
+    formed."""
     return native().penalize_logits(logits, tokens, lens, prompt_lens, repetition, frequency, presence, bias_ids, bias,
                                     allowed, int(vocab_offset), out, keys)

@@ -240,3 +240,57 @@ def test_outputs_written_in_place_raise_their_version(cuda):
         late = _calls(cuda)
     for call, _ in late.values():
         call()
+
+
+def test_gradients_that_are_not_formed_are_refused(cuda):
+    """Operators without a backward pass, and forward-mode tangents, raise where a derivative would be lost."""
+    import torch.autograd.forward_ad as fwd
+
+    cos, sin = K.rotary_tables(64, 64, device=cuda)
+    pos = torch.arange(2, dtype=torch.int32, device=cuda)
+    h = torch.randn(1, 2, 4, 64, device=cuda).half()
+    kc, vc = torch.randn(3, 2, 16, 64, device=cuda).half(), torch.randn(3, 2, 16, 64, device=cuda).half()
+    bt, cl = torch.arange(2, dtype=torch.int32, device=cuda).view(1, 2), torch.zeros(1, dtype=torch.int32, device=cuda)
+    qkv, w = torch.randn(1, 2, 8 * 64, device=cuda).half(), torch.ones(64, device=cuda).half()
+    L, one = torch.randn(2, 64, device=cuda), torch.ones(2, device=cuda)
+    tok = torch.zeros(2, 4, dtype=torch.int32, device=cuda)
+    ids, bias = torch.zeros(2, 1, dtype=torch.int32, device=cuda), torch.ones(2, 1, device=cuda)
+    x, x1, wf = torch.randn(2, 3, 64, device=cuda), torch.randn(2, 1, 64, device=cuda), torch.ones(64, device=cuda)
+
+    def tree(q=h, k=kc, v=vc):
+        return K.tree_attention(q, k, v, bt, cl, None, 0.1)
+
+    def append(qkv=qkv, wq=w, wk=w, b=qkv[0, 0].clone()):
+        return K.qk_norm_rotary_append_kv(qkv, pos, cos, sin, bt, cl, torch.empty_like(h), kc.clone(), vc.clone(), 4, 2,
+                                          q_weight=wq, k_weight=wk, bias=b)
+
+    def logits(x=L, rep=one, freq=one, pres=one, bias=bias):
+        return K.penalize_logits(x, tokens=tok, repetition=rep, frequency=freq, presence=pres, bias_ids=ids, bias=bias)
+
+    def back(dq=x, dk=x1, q=x, k=x1, wq=wf, wk=wf):
+        return K.qk_norm_rotary_backward(dq, dk, q, k, wq, wk, pos, cos, sin)
+
+    plain = [(tree, dict(q=h, k=kc, v=vc)), (append, dict(qkv=qkv, wq=w, wk=w, b=qkv[0, 0].clone())),
+             (logits, dict(x=L, rep=one, freq=one, pres=one, bias=bias))]
+    for fn, args in plain:
+        want = fn()
+        for name, t in args.items():
+            leaf = t.clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="no gradient"):
+                fn(**{name: leaf})
+            with torch.no_grad():
+                got = fn(**{name: leaf})
+            for a, b in zip(*((r if isinstance(r, tuple) else (r,)) for r in (got, want))):
+                assert torch.equal(a, b), (fn.__name__, name)
+    outs = dict(rotary=lambda x: K.rotary(x, pos, cos, sin), rotary_out=lambda x: K.rotary(x, pos, cos, sin, out=torch.empty(2, 3, 64, device=cuda)),
+                q=lambda x: K.qk_norm_rotary(x, x1, wf, wf, pos, cos, sin), k=lambda x: K.qk_norm_rotary(x1, x, wf, wf, pos, cos, sin),
+                w=lambda w: K.qk_norm_rotary(x, x1, w, wf, pos, cos, sin), logits=lambda x: logits(x=x), back=lambda q: back(q=q),
+                tree=lambda q: tree(q=q), append=lambda t: append(qkv=t))
+    give = dict(w=wf, logits=L, tree=h, append=qkv)
+    with fwd.dual_level():
+        for grad in (False, True):
+            for name, fn in outs.items():
+                t = give.get(name, x).clone().requires_grad_(grad)
+                dual = fwd.make_dual(t, torch.ones_like(t))
+                with pytest.raises(RuntimeError, match="forward-mode|no gradient"):
+                    fn(dual)

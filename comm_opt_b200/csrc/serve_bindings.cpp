@@ -378,8 +378,9 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
   COB_CHECK(qkv.stride(-1) == 1 || qkv.numel() == 0, "qkv's last dimension must be contiguous");
   const Tables t = tables(cos_t, sin_t, D, qkv);
   dense(positions, "positions", torch::kInt, qkv);
-  COB_CHECK(positions.numel() == B * S || (positions.dim() == 1 && positions.numel() == S),
-            "positions must be [batch, seq], [batch * seq] or [seq]");
+  const bool per_row = positions.dim() == 2 ? positions.size(0) == B && positions.size(1) == S
+                                            : positions.dim() == 1 && positions.size(0) == B * S;
+  COB_CHECK(per_row || (positions.dim() == 1 && positions.size(0) == S), "positions must be [batch, seq], [batch * seq] or [seq]");
   dense(q_out, "q_out", qkv.scalar_type(), qkv);
   COB_CHECK(q_out.numel() == B * S * nq * D, "q_out must hold batch x seq x nq x head_dim elements");
   cache_ok(k_cache, v_cache, block_tables, qkv, nkv, D, B);
@@ -433,7 +434,7 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
   p.out[0].heads = (int)nq;
   p.pos = positions.data_ptr<int32_t>();
   p.pos_ss = 1;
-  p.pos_sb = positions.numel() == B * S ? S : 0;
+  p.pos_sb = per_row ? S : 0;
   p.cos_t = cos_t.data_ptr<float>();
   p.sin_t = sin_t.data_ptr<float>();
   p.max_pos = t.max_pos;

@@ -294,3 +294,27 @@ def test_gradients_that_are_not_formed_are_refused(cuda):
                 dual = fwd.make_dual(t, torch.ones_like(t))
                 with pytest.raises(RuntimeError, match="forward-mode|no gradient"):
                     fn(dual)
+
+
+# ------------------------------------------------------------------------------------------------ arguments
+def test_append_takes_positions_by_batch_and_sequence_only(cuda):
+    """[seq, batch] positions hold as many numbers and would rotate every row by another's."""
+    cos, sin = K.rotary_tables(64, 64, device=cuda)
+    B, S, nq, nkv = 2, 3, 2, 1
+    qkv = torch.randn(B, S, 4 * 64, device=cuda)
+    bt, st = torch.arange(4, dtype=torch.int32, device=cuda).view(B, 2), torch.zeros(B, dtype=torch.int32, device=cuda)
+    pos = torch.arange(6, dtype=torch.int32, device=cuda).view(B, S)
+
+    def call(p, x=qkv):
+        q, k, v = (torch.zeros(s, device=cuda) for s in ((B, S, nq, 64), (4, nkv, 16, 64), (4, nkv, 16, 64)))
+        K.qk_norm_rotary_append_kv(x, p, cos, sin, bt, st, q, k, v, nq, nkv)
+        return q, k, v
+
+    want = call(pos)
+    for same in (call(pos.flatten()), call(pos, qkv.flatten(0, 1)), call(pos.flatten(), qkv.flatten(0, 1))):
+        assert all(torch.equal(a, b) for a, b in zip(same, want))
+    row = torch.arange(S, dtype=torch.int32, device=cuda)
+    assert all(torch.equal(a, b) for a, b in zip(call(row), call(row.expand(B, S).contiguous())))
+    for p in (pos.t().contiguous(), pos[None], pos[:, :, None], pos[:, None], row[None], pos.flatten()[:, None]):
+        with pytest.raises(RuntimeError, match="positions"):
+            call(p)

@@ -4,6 +4,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cmath>
 #include <initializer_list>
 #include <tuple>
 #include <utility>
@@ -463,6 +464,7 @@ Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_
   COB_CHECK(dtype != cob::kF32, "q and the caches must be float16 or bfloat16");
   constants("tree_attention", {&q, &k_cache, &v_cache, given(out)});
   COB_CHECK(timeout_ns >= 0, "timeout_ms must not be negative");
+  COB_CHECK(std::isfinite((float)scale), "scale must be finite");
   cob::TreeAttnParams p;
   const int64_t B = q.size(0), T = q.size(1), nq = q.size(2), D = q.size(3);
   COB_CHECK(D == 64 || D == 128, "head_dim must be 64 or 128, got ", D);

@@ -318,3 +318,10 @@ def test_append_takes_positions_by_batch_and_sequence_only(cuda):
     for p in (pos.t().contiguous(), pos[None], pos[:, :, None], pos[:, None], row[None], pos.flatten()[:, None]):
         with pytest.raises(RuntimeError, match="positions"):
             call(p)
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e60])
+def test_tree_attention_refuses_a_scale_that_is_not_finite(cuda, scale):
+    q, kc, vc, bt, cl, bits = make_tree(gen(cuda, 1), cuda, 1, 3, 2, 1, 64, [20], torch.float16)
+    with pytest.raises(RuntimeError, match="scale"):
+        K.tree_attention(q, kc, vc, bt, cl, bits, scale)

@@ -10,8 +10,8 @@
 // the softmax. S is written by the tensor cores into one of a row tile's two TMEM buffers, P goes back over it in 16 bits
 // and is the A operand of P V straight from TMEM; O stays in TMEM. Q K^T of the next step runs while the softmax works
 // on this one, which is what two buffers of 64 columns per row tile are for (one of 128 left the softmax waiting 1 us a
-// tile for its scores). O is rescaled only where a row's maximum rose by more than 2^8 (P stays below 2^8, far inside the
-// 16-bit types; O / l is the same number), which after the first tiles hardly happens.
+// tile for its scores). O is rescaled only where a row's maximum rose by more than 2^8 (bf16; fp16 2^4, see kRise), which
+// after the first tiles hardly happens; O / l is the same number.
 //
 // Work is cut into equal shares of the flattened (sequence, KV head, tile) space by the sequences' actual lengths,
 // each (sequence, KV head) charged two tiles for its start and end, so ragged batches and few long sequences both fill
@@ -165,6 +165,21 @@ template <typename T>
 constexpr uint32_t kExpMask = 0x7C00u;  // exponent bits of __half: all set in infinities and NaN
 template <>
 constexpr uint32_t kExpMask<__nv_bfloat16> = 0x7F80u;
+
+// Weights are P = 2^(x + kShift), x relative to a reference maximum that lies at most kRise below the row's (and both cancel in
+// O / l). They are rounded to the cache's 16 bits, which is what the tensor cores take beside a 16-bit V: at most half a step
+// each, of numbers that the sum l counts in fp32. bf16 has fp32's range. fp16 ends at 2^16 and loses bits below 2^-14, so its
+// weights sit as high as they can: they are normal numbers from 2^-25 of the row's largest on (without the shift from 2^-14 on,
+// and nothing below 2^-25: 4000 tokens at 2^-26 behind one strong token vanished from O while l counted them). The smaller kRise
+// costs a rescaling of O now and then.
+template <typename T>
+constexpr float kRise = 4.f;
+template <typename T>
+constexpr float kShift = 11.f;
+template <>
+constexpr float kRise<__nv_bfloat16> = 8.f;
+template <>
+constexpr float kShift<__nv_bfloat16> = 0.f;
 
 // zeroes the non-finite halves of a vector; non-zero if there were any
 template <typename T>
@@ -617,7 +632,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
             }
           float mn = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
           if (mn == INFINITY) mn = __uint_as_float(0x7fc00000u);  // inf - inf
-          const bool rise = st == 0 || !((mn - m) * c <= 8.f);
+          const bool rise = st == 0 || !((mn - m) * c <= kRise<T>);
           const float f = !rise || mn == m ? 1.f : ex2((m - mn) * c);
           if (rise) m = mn;  // (by row: no row's result depends on another's)
           l *= f;
@@ -637,7 +652,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
           }
           okay = my_turn(n);
           if (!okay) break;
-          const float mu = m == -INFINITY ? 0.f : m * c;
+          const float mu = m == -INFINITY ? 0.f : m * c - kShift<T>;
           const uint64_t c2 = pair(c, c), mu2 = pair(-mu, -mu);
           uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll

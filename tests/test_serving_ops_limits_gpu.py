@@ -325,3 +325,31 @@ def test_tree_attention_refuses_a_scale_that_is_not_finite(cuda, scale):
     q, kc, vc, bt, cl, bits = make_tree(gen(cuda, 1), cuda, 1, 3, 2, 1, 64, [20], torch.float16)
     with pytest.raises(RuntimeError, match="scale"):
         K.tree_attention(q, kc, vc, bt, cl, bits, scale)
+
+
+# --------------------------------------------------------------------------------------------- small weights
+@pytest.mark.parametrize("D,T,G", [(64, 1, 1), (128, 3, 2), (64, 64, 4)])
+@pytest.mark.parametrize("bits", [12, 20, 26, 30])
+def test_tree_attention_weights_behind_one_strong_token(cuda, D, T, G, bits):
+    """One token with weight 1 and v = 0, 4000 tokens with weights of 2^-bits and v = 1 (fp16), heads enough for each to be
+    walked whole by one CTA: the many are what the row says, although each weight is far below the strong one's step.
+
+    A weight is held as fp16(2^11 w), w relative to the row's reference maximum, which is at most 2^4 below the true one:
+    normal numbers (half a step of the type) down to w = 2^-25, below that off by at most 2^-25 / 2^11 = 2^-36 each."""
+    B, nkv, n, dtype = 6, 64, 4001, torch.float16
+    pages = (n + T + 15) // 16
+    kc = torch.zeros(B * pages, nkv, 16, D, device=cuda, dtype=dtype)
+    vc = torch.ones(B * pages, nkv, 16, D, device=cuda, dtype=dtype)
+    bt = torch.arange(B * pages, device=cuda, dtype=torch.int32).view(B, pages)
+    kc[bt[:, 0].long(), :, 5, 0], vc[bt[:, 0].long(), :, 5] = bits, 0.0  # exact in the type; the score is bits * ln 2
+    q = torch.zeros(B, T, nkv * G, D, device=cuda, dtype=dtype)
+    q[..., 0] = 1.0
+    cl = torch.full((B,), n, device=cuda, dtype=torch.int32)
+    mask = torch.zeros(T, dtype=torch.int64, device=cuda)  # no drafted token sees another or itself
+    y = K.tree_attention(q, kc, vc, bt, cl, mask, math.log(2.0))
+    many = (n - 1) * 2.0 ** -bits
+    ref = torch.full_like(y, many / (1 + many), dtype=torch.float64)
+    # the score's error: one rounding of the scale and of the product, each of bits * ln 2; sums over n slots in fp32;
+    # each weight's rounding, and the absolute one below the normal numbers
+    err = ref * (2 * (D + 8) * F32U * bits + (n + 32) * F32U + u(dtype)) + (n - 1) * 2.0 ** -36
+    close(y, ref, err)

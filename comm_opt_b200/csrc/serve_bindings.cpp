@@ -44,21 +44,37 @@ void dense(const Tensor& t, const char* n, torch::ScalarType ty, const Tensor& r
   COB_CHECK(t.is_contiguous(), n, " must be contiguous");
 }
 
-// first byte and the one past the last that a tensor's elements reach
-std::pair<uintptr_t, uintptr_t> bytes_of(const Tensor& t) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr());
-  int64_t last = 0;
-  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-  return {a, a + (last + 1) * t.element_size()};
-}
-bool overlap(const Tensor& a, const Tensor& b) {
-  if (a.numel() == 0 || b.numel() == 0) return false;
-  const auto x = bytes_of(a), y = bytes_of(b);
-  return x.first < y.second && y.first < x.second;
-}
-// what a call writes lies apart from all of the others
-void apart(const Tensor& t, const char* n, std::initializer_list<const Tensor*> others) {
-  for (const Tensor* o : others) COB_CHECK(!o || !overlap(t, *o), n, " must lie in memory of its own: it overlaps another operand");
+// the bytes that a tensor's elements reach
+struct Span {
+  uintptr_t lo = 0, hi = 0;
+  Span() = default;
+  explicit Span(const Tensor* t) {
+    if (!t || t->numel() == 0) return;
+    lo = reinterpret_cast<uintptr_t>(t->const_data_ptr());
+    int64_t last = t->numel() - 1;
+    if (!t->is_contiguous()) {
+      const auto n = t->sizes(), s = t->strides();
+      last = 0;
+      for (size_t i = 0; i < n.size(); ++i) last += (n[i] - 1) * s[i];
+    }
+    hi = lo + (last + 1) * t->element_size();
+  }
+  bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
+};
+bool overlap(const Tensor& a, const Tensor& b) { return Span(&a).meets(Span(&b)); }
+// what a call writes lies apart from what it reads, and from whatever else it writes
+void apart(std::initializer_list<const Tensor*> written, std::initializer_list<const Tensor*> read, const char* what) {
+  Span w[4];
+  int n = 0;
+  for (const Tensor* t : written) {
+    w[n] = Span(t);
+    for (int i = 0; i < n; ++i) COB_CHECK(!w[n].meets(w[i]), what);
+    ++n;
+  }
+  for (const Tensor* t : read) {
+    const Span r(t);
+    for (int i = 0; i < n; ++i) COB_CHECK(!w[i].meets(r), what);
+  }
 }
 const Tensor* given(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }
 
@@ -174,7 +190,7 @@ Tensor py_rotary(Tensor x, Tensor positions, Tensor cos_t, Tensor sin_t, bool in
     writable(y, "out");
     const bool in_place = y.data_ptr() == x.data_ptr() && y.strides() == x.strides();
     COB_CHECK(in_place || !overlap(x, y), "out must be x itself or lie in memory of its own");
-    apart(y, "out", {&positions, &cos_t, &sin_t});
+    apart({&y}, {&positions, &cos_t, &sin_t}, "out must lie in memory of its own: it overlaps an input");
   }
   const c10::cuda::CUDAGuard g(x.device());
   if (!out.has_value()) y = torch::empty(x.sizes(), x.options().requires_grad(false));
@@ -385,12 +401,9 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
   dense(q_out, "q_out", qkv.scalar_type(), qkv);
   COB_CHECK(q_out.numel() == B * S * nq * D, "q_out must hold batch x seq x nq x head_dim elements");
   cache_ok(k_cache, v_cache, block_tables, qkv, nkv, D, B);
-  COB_CHECK(!overlap(q_out, qkv) && !overlap(k_cache, qkv) && !overlap(v_cache, qkv) && !overlap(q_out, k_cache) &&
-                !overlap(q_out, v_cache) && !overlap(k_cache, v_cache),
-            "q_out and the caches must lie in memory of their own");
-  const std::pair<const Tensor*, const char*> outs[3] = {{&q_out, "q_out"}, {&k_cache, "k_cache"}, {&v_cache, "v_cache"}};
-  for (const auto& w : outs)
-    apart(*w.first, w.second, {&positions, &cos_t, &sin_t, &block_tables, &starts, given(wq), given(wk), given(lens), given(bias)});
+  apart({&q_out, &k_cache, &v_cache},
+        {&qkv, &positions, &cos_t, &sin_t, &block_tables, &starts, given(wq), given(wk), given(lens), given(bias)},
+        "q_out and the caches must lie in memory of their own");
   COB_CHECK(wq.has_value() == wk.has_value(), "give both norm weights or neither");
   cob::RotaryParams p;
   Tensor like = qkv;  // type and device of the operands; head_dim components
@@ -454,7 +467,7 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
   p.num_blocks = (int)k_cache.size(0);
   p.dtype = code_of(qkv, "qkv");
   ok(cob::rotary_forward(p, cur()), "qk_norm_rotary_append_kv");
-  for (const auto& w : outs) written(*w.first);
+  for (const Tensor* t : {&q_out, &k_cache, &v_cache}) written(*t);
 }
 
 Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor ctx_lens, OptTensor mask,
@@ -499,7 +512,7 @@ Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_
     COB_CHECK(y.sizes() == q.sizes() && y.scalar_type() == q.scalar_type(), "out must have q's shape and type");
     COB_CHECK(y.numel() == 0 || vec_ok(y), "out's heads must be contiguous and 16-byte aligned");
     writable(y, "out");
-    apart(y, "out", {&q, &k_cache, &v_cache, &block_tables, &ctx_lens, given(mask), given(tree_lens)});
+    apart({&y}, {&q, &k_cache, &v_cache, &block_tables, &ctx_lens, given(mask), given(tree_lens)}, "out must lie in memory of its own");
   } else {
     // rows past tree_lens are not written: give them a value
     y = tree_lens.has_value() ? torch::zeros(q.sizes(), q.options()) : torch::empty(q.sizes(), q.options());
@@ -620,13 +633,12 @@ Tensor py_penalize_logits(Tensor logits, OptTensor tokens, OptTensor lens, OptTe
   } else {
     y = torch::empty(logits.sizes(), logits.options());
   }
-  const std::initializer_list<const Tensor*> inputs = {given(tokens),   given(lens),     given(prompt_lens), given(repetition), given(frequency),
-                                                       given(presence), given(bias_ids), given(bias),        given(allowed)};
-  if (out.has_value()) apart(y, "out", inputs);
-  if (keys.has_value()) {
-    apart(*keys, "keys", inputs);
-    apart(*keys, "keys", {&logits, &y});
-  }
+  if (out.has_value() || keys.has_value())
+    apart({out.has_value() ? &y : nullptr, given(keys)},
+          {given(tokens), given(lens), given(prompt_lens), given(repetition), given(frequency), given(presence), given(bias_ids),
+           given(bias), given(allowed)},
+          "out and keys must lie in memory of their own");
+  if (keys.has_value()) COB_CHECK(!overlap(*keys, logits), "keys must lie in memory of their own");
   if (B == 0) return y;
   p.logits = logits.data_ptr();
   p.out = y.data_ptr();

@@ -103,6 +103,14 @@ struct Vec<__nv_bfloat16> {
   }
 };
 
+// Greedy argmax key: order-preserving 32-bit image of the value in the high word, inverted index in the low word, so
+// the maximum key is the largest value and, among equal values, the lowest index (-0 equals +0: the sum with +0 is +0).
+__device__ __forceinline__ unsigned long long greedy_key(float v, uint32_t idx) {
+  uint32_t u = __float_as_uint(v + 0.f);
+  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return ((unsigned long long)u << 32) | (0xFFFFFFFFu - idx);
+}
+
 // ---------------------------------------------------------------------------------------------
 // Lamport-style "value carries its own arrival" encoding.
 //

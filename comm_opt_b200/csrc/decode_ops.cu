@@ -148,13 +148,6 @@ __global__ void k_silu_mul(const T* __restrict__ gu, T* __restrict__ out, int in
   }
 }
 
-// Greedy argmax key: order-preserving 32-bit image of the value in the high word, inverted index in
-// the low word, so the maximum key is the largest value and, among equal values, the lowest index.
-__device__ __forceinline__ unsigned long long amax_key(float v, uint32_t idx) {
-  uint32_t u = __float_as_uint(v);
-  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return ((unsigned long long)u << 32) | (0xFFFFFFFFu - idx);
-}
 __device__ __forceinline__ unsigned long long umax64(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
 
 constexpr int kArgmaxChunk = 2048;
@@ -169,7 +162,7 @@ __global__ void __launch_bounds__(256) k_argmax_local(const T* __restrict__ logi
   const int i0 = blockIdx.y * kArgmaxChunk, i1 = min(vocab, i0 + kArgmaxChunk);
   const T* lr = logits + (size_t)row * vocab;
   unsigned long long best = 0ull;
-  for (int i = i0 + threadIdx.x; i < i1; i += blockDim.x) best = umax64(best, amax_key(to_f(lr[i]), i + vocab_offset));
+  for (int i = i0 + threadIdx.x; i < i1; i += blockDim.x) best = umax64(best, greedy_key(to_f(lr[i]), i + vocab_offset));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = umax64(best, __shfl_xor_sync(0xffffffffu, best, o));
   __shared__ unsigned long long sk[8];

@@ -21,12 +21,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr uint32_t kInPrompt = 0x80000000u;
 
-__device__ __forceinline__ unsigned long long greedy_key(float v, uint32_t idx) {
-  uint32_t u = __float_as_uint(v);
-  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return ((unsigned long long)u << 32) | (0xFFFFFFFFu - idx);
-}
-
 // The row's scalars, and one id's chain of roundings. Products and differences are rounded one by one (no fused
 // multiply-add), so the result is that of the same formula written in elementwise fp32 operations.
 struct RowScalars {

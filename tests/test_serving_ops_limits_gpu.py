@@ -353,3 +353,17 @@ def test_tree_attention_weights_behind_one_strong_token(cuda, D, T, G, bits):
     # each weight's rounding, and the absolute one below the normal numbers
     err = ref * (2 * (D + 8) * F32U * bits + (n + 32) * F32U + u(dtype)) + (n - 1) * 2.0 ** -36
     close(y, ref, err)
+
+
+# --------------------------------------------------------------------------------------------- greedy choice
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_greedy_choice_takes_the_lowest_of_equal_zeros(cuda, dtype):
+    """-0 and +0 are equal: the lowest id wins, in argmax_local and in the penalties' keys."""
+    x = torch.full((3, 300), -1.0, device=cuda, dtype=dtype)
+    x[0, 7], x[0, 8], x[0, 290] = -0.0, 0.0, 0.0
+    x[1, 100], x[1, 101] = 0.0, -0.0
+    x[2, 299], x[2, 298] = 0.0, -0.0
+    keys = torch.zeros(3, dtype=torch.int64, device=cuda)
+    y = K.penalize_logits(x, keys=keys)
+    assert torch.equal(y, x) and torch.equal(keys, K.argmax_local(x, 0))
+    assert K.argmax_combine(keys.view(1, 3), 1).tolist() == [7, 100, 298] == x.float().argmax(-1).tolist()

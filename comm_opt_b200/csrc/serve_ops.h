@@ -28,7 +28,7 @@ struct RotaryParams {
   const float* sin_t = nullptr;
   int max_pos = 0, rot = 0, D = 0, batch = 0, seq = 0;
   int interleaved = 0;  // pairs (2j, 2j + 1); else (j, j + rot / 2)
-  int inverse = 0;      // rotate by the negative angle (the gradient of a rotation)
+  int inverse = 0;      // the transpose: sines negated (the gradient of a rotation)
   float eps = 0.f;
   // append form
   int append = 0;

@@ -70,7 +70,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: tor
     """Rotate x [tokens, heads, D] or [batch, seq, heads, D] (fp32, fp16, bf16; any strides) by its positions
     (int32 [seq] or [batch, seq]) and the tables cos, sin (fp32 [max_pos, rotary_dim / 2], see `rotary_tables`).
 
-    Differentiable in x (reverse mode). ``inverse`` rotates back. ``out`` may be x (in place, no gradient) or other memory. A row whose
+    Differentiable in x (reverse mode). ``inverse`` applies the transpose, the gradient's rotation: it rotates back
+    where cos^2 + sin^2 = 1, and with tables that carry a factor m (YaRN's attention_factor) leaves m^2 x. ``out`` may be x (in place, no gradient) or other memory. A row whose
     position lies outside the tables becomes zeros (and has a zero gradient): padded rows carry position -1."""
     if out is None and x.requires_grad and torch.is_grad_enabled():
         return native().rotary_autograd(x, positions, cos, sin, bool(interleaved), bool(inverse))

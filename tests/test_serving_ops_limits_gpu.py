@@ -367,3 +367,28 @@ def test_greedy_choice_takes_the_lowest_of_equal_zeros(cuda, dtype):
     y = K.penalize_logits(x, keys=keys)
     assert torch.equal(y, x) and torch.equal(keys, K.argmax_local(x, 0))
     assert K.argmax_combine(keys.view(1, 3), 1).tolist() == [7, 100, 298] == x.float().argmax(-1).tolist()
+
+
+# -------------------------------------------------------------------------------------------------- transposes
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_inverse_is_the_transpose_also_of_scaled_tables(cuda, interleaved):
+    """YaRN tables carry a factor m: rotating and rotating back multiplies by m^2; the gradient is the transpose."""
+    g = gen(cuda, 13)
+    cos, sin = K.rotary_tables(40, 32, 1e4, dict(type="yarn", factor=16.0, original=20), device=cuda)
+    m2 = (0.1 * math.log(16.0) + 1.0) ** 2
+    pos = torch.arange(9, device=cuda, dtype=torch.int32)
+    x = randn(g, 2, 9, 3, 64).requires_grad_()
+    y = K.rotary(x, pos, cos, sin, interleaved=interleaved)
+    dy = randn(g, 2, 9, 3, 64)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    back = K.rotary(dy, pos, cos, sin, interleaved=interleaved, inverse=True)
+    assert torch.equal(dx, back)
+    ref, mag = rotate64(dy.double(), cos[:9], sin[:9], interleaved, -1.0)
+    close(back, ref, 3 * F32U * mag)
+    round_trip = K.rotary(y.detach(), pos, cos, sin, interleaved=interleaved, inverse=True).double()
+    want = x.detach().double().clone()
+    a, b = ((slice(0, 32, 2), slice(1, 32, 2)) if interleaved else (slice(0, 16), slice(16, 32)))
+    want[..., a] *= m2
+    want[..., b] *= m2
+    big = float(x.detach().abs().max()) * 2 * m2
+    assert float((round_trip - want).abs().max()) <= 12 * F32U * big

@@ -392,3 +392,224 @@ def test_inverse_is_the_transpose_also_of_scaled_tables(cuda, interleaved):
     want[..., b] *= m2
     big = float(x.detach().abs().max()) * 2 * m2
     assert float((round_trip - want).abs().max()) <= 12 * F32U * big
+
+
+# -------------------------------------------------------------- forms that only many rows select (rotary.cu's launchers)
+SMS = 148
+
+
+def _lanes(D, V):
+    gl = 1
+    while gl < 32 and gl < D // (2 * V):
+        gl *= 2
+    return gl
+
+
+def _forward_form(rows, heads, D, steps):
+    """(several heads a lane, head blocks that a warp takes, whether the last step of the widest operand is partial)"""
+    per = 32 // _lanes(D, 8)
+    many = rows * sum(heads) >= SMS * 64 * per
+    blocks = [-(-h // (per * steps)) for h in heads]
+    inner = max(1, min(sum(blocks), rows * sum(blocks) // (SMS * 32)))
+    return many, inner, heads[0] % (per * steps) != 0
+
+
+def _dw_chain(rows, heads, other, D, V, hpt):
+    """The longest chain of additions behind a weight's gradient: a lane's rows and heads, lanes, warps, blocks."""
+    cost = (heads + 12, other + 12)
+    nb = max(1, min(SMS * 3 * cost[0] // sum(cost), rows * ((heads + 7) // 8)))
+    per = 32 // _lanes(D, V)
+    inner = 4 if rows >= SMS * 24 else 1
+    groups = -(-(-(-heads // (per * hpt))) // inner)
+    units = -(-rows * groups // (nb * 4))
+    return units * inner * hpt + 5 + 4 + -(-nb // 32) + 5
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,S,H,D,rot", [(8, 512, 40, 128, 64), (3, 1111, 37, 128, 128), (1, 4001, 50, 64, 64), (2, 2000, 21, 256, 64)])
+def test_rotary_of_many_rows(cuda, interleaved, dtype, B, S, H, D, rot):
+    many, inner, partial = _forward_form(B * S, (H,), D, 3)
+    assert many and inner > 1 and partial
+    g = gen(cuda, S)
+    cos, sin = K.rotary_tables(300, rot, 1e4, device=cuda)
+    pos = torch.randint(0, 300, (B, S), generator=g, device=cuda, dtype=torch.int32)
+    pos[0, 5], pos[-1, -1] = -1, 300
+    wide = randn(g, B, S, H + 2, D, dtype=dtype)
+    x = wide[:, :, 1:H + 1]
+    p = pos.long().clamp(0, 299)
+    pad = (pos < 0) | (pos >= 300)
+    for inverse in (False, True):
+        ref, mag = rotate64(x.double(), cos[p], sin[p], interleaved, -1.0 if inverse else 1.0)
+        ref[pad], mag[pad] = 0, 0
+        y = K.rotary(x, pos, cos, sin, interleaved=interleaved, inverse=inverse)
+        close(y, ref, 3 * F32U * mag)
+        z = wide.clone()
+        K.rotary(z[:, :, 1:H + 1], pos, cos, sin, interleaved=interleaved, inverse=inverse, out=z[:, :, 1:H + 1])
+        assert torch.equal(z[:, :, 1:H + 1], y) and torch.equal(z[:, :, 0], wide[:, :, 0]) and torch.equal(z[:, :, -1], wide[:, :, -1])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,S,nq,nk,D,rot", [(4, 2048, 37, 5, 128, 128), (2, 1000, 37, 5, 128, 64), (1, 3553, 40, 8, 128, 128),
+                                             (2, 4100, 5, 1, 64, 64), (3, 1300, 21, 3, 64, 32)])
+def test_qk_norm_rotary_of_many_rows(cuda, interleaved, dtype, B, S, nq, nk, D, rot):
+    rows = B * S
+    many, inner, _ = _forward_form(rows, (nq, nk), D, 2)
+    assert many == (nq > 5) and (not many or inner > 1)
+    g = gen(cuda, S + nq)
+    cos, sin = K.rotary_tables(300, rot, 1e4, device=cuda)
+    pos = torch.randint(0, 300, (B, S), generator=g, device=cuda, dtype=torch.int32)
+    pos[0, 3], pos[-1, S // 2] = -1, 300
+    pad = (pos < 0) | (pos >= 300)
+    live = ~pad
+    p = pos.long().clamp(0, 299)
+    c, s = cos[p][live], sin[p][live]
+    qkv = randn(g, B, S, nq + 2 * nk, D, dtype=dtype, std=2.0)
+    qkv[pad] = float("nan")  # what padding may hold
+    q, k = qkv[:, :, :nq].detach().requires_grad_(), qkv[:, :, nq:nq + nk].detach().requires_grad_()
+    wq, wk = (1 + 0.2 * randn(g, D)).requires_grad_(), (1 + 0.2 * randn(g, D)).requires_grad_()
+    ys = K.qk_norm_rotary(q, k, wq, wk, pos, cos, sin, 1e-6, interleaved=interleaved)
+    for y, x, w in zip(ys, (q, k), (wq, wk)):
+        ref, mag = norm_rotate64(x.detach()[live], w.detach(), c, s, 1e-6, interleaved)
+        close(y.detach()[live], ref, (D + 10) * F32U * torch.maximum(mag, ref.abs()))
+        assert not bool(y[pad].any())
+    for sparse in (False, True):  # all rows; then a few rows and heads only, so that none of them can be missing from dw
+        dys = [randn(g, *y.shape, dtype=dtype) for y in ys]
+        if sparse:
+            dys = [d * (torch.rand(d.shape[:3], generator=g, device=cuda) < 40 / (rows * d.shape[2]))[..., None] for d in dys]
+        for d in dys:
+            d[pad] = float("nan")
+        grads = torch.autograd.grad(ys, (q, k, wq, wk), dys, retain_graph=True)
+        again = K.qk_norm_rotary_backward(*dys, q, k, wq, wk, pos, cos, sin, 1e-6, interleaved=interleaved)
+        assert all(torch.equal(a, b) for a, b in zip(grads, again))  # a fixed order of the sums
+        for i, (x, w) in enumerate(((q, wq), (k, wk))):
+            dx, mag, dw, wmag = norm_rotate_grad64(x.detach()[live], w.detach(), dys[i][live], c, s, 1e-6, interleaved)
+            close(grads[i][live], dx, (3 * D + 20) * F32U * mag)
+            assert not bool(grads[i][pad].any())
+            n = _dw_chain(rows, x.shape[2], (nk, nq)[i], D, 8, 2)
+            close(grads[2 + i], dw, (n + D + 20) * F32U * wmag)
+
+
+@pytest.mark.parametrize("dtype,D,rot,off", [(torch.bfloat16, 80, 20, 0), (torch.float16, 96, 24, 0), (torch.float32, 80, 20, 0),
+                                             (torch.bfloat16, 64, 64, 1)])
+def test_qk_norm_rotary_of_many_narrow_rows(cuda, dtype, D, rot, off):
+    """Vectors that the layout or the alignment keeps narrow, with rows enough for four head blocks a warp."""
+    B, S, nq, nk = 2, 1900, 5, 2
+    assert B * S >= SMS * 24
+    g = gen(cuda, D + off)
+    cos, sin = K.rotary_tables(S, rot, 1e4, device=cuda)
+    pos = torch.arange(S, device=cuda, dtype=torch.int32)
+
+    def operand(h):
+        flat = torch.empty(B * S * h * D + off, device=cuda, dtype=dtype)
+        return flat[off:].view(B, S, h, D).copy_(randn(g, B, S, h, D, dtype=dtype))
+
+    q, k, dq, dk = operand(nq), operand(nk), operand(nq), operand(nk)
+    wq, wk = 1 + 0.2 * randn(g, D), 1 + 0.2 * randn(g, D)
+    ys = K.qk_norm_rotary(q, k, wq, wk, pos, cos, sin)
+    grads = K.qk_norm_rotary_backward(dq, dk, q, k, wq, wk, pos, cos, sin)
+    for i, (x, w, d) in enumerate(((q, wq, dq), (k, wk, dk))):
+        ref, mag = norm_rotate64(x, w, cos[None, :S], sin[None, :S], 1e-6, False)
+        close(ys[i], ref, (D + 10) * F32U * torch.maximum(mag, ref.abs()))
+        dx, mag, dw, wmag = norm_rotate_grad64(x, w, d, cos[None, :S], sin[None, :S], 1e-6, False)
+        close(grads[i], dx, (3 * D + 20) * F32U * mag)
+        close(grads[2 + i], dw, (_dw_chain(B * S, x.shape[2], (nk, nq)[i], D, 1, 1) + D + 20) * F32U * wmag)
+
+
+@pytest.mark.parametrize("interleaved,norm,bias", [(False, True, True), (True, True, False), (False, False, True), (True, False, False)])
+@pytest.mark.parametrize("dtype,B,S,nq,nkv,D,rot", [(torch.bfloat16, 4, 2048, 40, 8, 128, 128), (torch.float16, 3, 1111, 37, 5, 128, 64),
+                                                    (torch.bfloat16, 5, 901, 21, 7, 64, 64)])
+def test_append_of_many_rows(cuda, interleaved, norm, bias, dtype, B, S, nq, nkv, D, rot):
+    many, inner, partial = _forward_form(B * S, (nq, nkv, nkv), D, 2 if norm else 3)
+    assert many and inner > 1 and partial == (nq != 40 or not norm)
+    g = gen(cuda, S + D)
+    n, pages = nq + 2 * nkv, (S + 40 + 15) // 16
+    cos, sin = K.rotary_tables(S + 60, rot, 1e4, device=cuda)
+    qkv = randn(g, B, S, n * D + 16, dtype=dtype)[..., :n * D]
+    starts = torch.randint(0, 41, (B,), generator=g, device=cuda, dtype=torch.int32)
+    lens = torch.randint(1, S + 1, (B,), generator=g, device=cuda, dtype=torch.int32)
+    lens[0], lens[1] = S, 0
+    pos = torch.randint(0, S + 60, (B, S), generator=g, device=cuda, dtype=torch.int32)
+    pos[0, 7] = -1
+    bt = torch.randperm(B * pages, generator=g, device=cuda).to(torch.int32).view(B, pages)
+    kc, vc = (randn(g, B * pages, nkv, 16, D, dtype=dtype) for _ in range(2))
+    wq, wk = (1 + 0.1 * randn(g, D)).to(dtype), (1 + 0.1 * randn(g, D)).to(dtype)
+    bv = randn(g, n * D, dtype=dtype) if bias else None
+    q_out = torch.full((B, S, nq, D), 3.0, device=cuda, dtype=dtype)
+    k1, v1 = kc.clone(), vc.clone()
+    K.qk_norm_rotary_append_kv(qkv, pos, cos, sin, bt, starts, q_out, k1, v1, nq, nkv, q_weight=wq if norm else None,
+                               k_weight=wk if norm else None, eps=1e-5, lens=lens, bias=bv, interleaved=interleaved)
+    live = (torch.arange(S, device=cuda)[None] < lens[:, None]) & (pos >= 0)
+    x = (qkv.double() + (bv.double() if bias else 0)).view(B, S, n, D)[live]
+    c, s = cos[pos[live].long()], sin[pos[live].long()]
+    b, row = live.nonzero().T
+    slot = starts.long()[b] + row
+    page, at = bt[b, slot // 16].long(), slot % 16
+    # a bias enters with one more rounding, of terms as large as |x| + |bias| <= 2 max
+    extra = 12 * F32U * (float(x.abs().max()) + 1) if bias else 0
+    n32 = ((D + 14) if norm else 4) * F32U
+    for got, part, w in ((q_out[live], x[:, :nq], wq), (k1[page, :, at], x[:, nq:nq + nkv], wk)):
+        ref, mag = norm_rotate64(part, w, c, s, 1e-5, interleaved) if norm else rotate64(part, c, s, interleaved)
+        close(got, ref, n32 * torch.maximum(mag, ref.abs()) + extra)
+    close(v1[page, :, at], x[:, nq + nkv:], extra)
+    assert bool((q_out[~live] == 3).all())
+    rest = torch.ones(B * pages, 16, dtype=torch.bool, device=cuda)
+    rest[page, at] = False
+    rest = rest[:, None].expand(-1, nkv, -1)
+    assert torch.equal(k1[rest], kc[rest]) and torch.equal(v1[rest], vc[rest])
+
+
+def test_qk_norm_rotary_gradients_of_one_output(cuda):
+    """Only one of the two outputs used: the other's gradients are zeros."""
+    g = gen(cuda, 2)
+    cos, sin = K.rotary_tables(9, 64, device=cuda)
+    pos = torch.arange(9, device=cuda, dtype=torch.int32)
+    t = [randn(g, 2, 9, 4, 64), randn(g, 2, 9, 2, 64), 1 + randn(g, 64), 1 + randn(g, 64)]
+    dys = [randn(g, 2, 9, 4, 64), randn(g, 2, 9, 2, 64)]
+    whole = K.qk_norm_rotary_backward(*dys, *t, pos, cos, sin)
+    for one in (0, 1):
+        leaves = [v.clone().requires_grad_() for v in t]
+        y = K.qk_norm_rotary(*leaves, pos, cos, sin)[one]
+        grads = torch.autograd.grad(y, leaves, dys[one])
+        for i in range(4):
+            assert torch.equal(grads[i], whole[i] if i % 2 == one else torch.zeros_like(whole[i])), (one, i)
+
+
+# -------------------------------------------------------------------------------------- large tree attentions
+def test_tree_attention_of_several_launches(cuda):
+    """300 sequences are three launches that share one workspace; contexts long enough that pieces are cut in each. Every
+    row against its 64-bit statement, and the same bits under programmatic launch, where they follow closely."""
+    g = gen(cuda, 31)
+    B, T, nq, nkv, D = 300, 3, 8, 2, 64
+    q, kc, vc, bt, _, bits = make_tree(g, cuda, B, T, nq, nkv, D, [900], torch.bfloat16)
+    ctx = torch.randint(0, 900, (B,), generator=g, device=cuda, dtype=torch.int32)
+    tl = torch.randint(0, T + 1, (B,), generator=g, device=cuda, dtype=torch.int32)
+    out = torch.full_like(q, 4.0)
+    K.tree_attention(q, kc, vc, bt, ctx, bits, 0.2, tree_lens=tl, out=out)
+    ref, mag, sm = tree_ref(q, kc, vc, bt, ctx, bits.tolist(), 0.2, tl)
+    check_tree(out, ref, mag, sm, 903, D)
+    dead = torch.arange(T, device=cuda)[None] >= tl[:, None]
+    assert bool((out[dead] == 4).all())
+    old = K.set_pdl(True)
+    try:
+        outs = [torch.full_like(q, 4.0) for _ in range(10)]
+        for o in outs:
+            K.tree_attention(q, kc, vc, bt, ctx, bits, 0.2, tree_lens=tl, out=o)
+        torch.cuda.synchronize()
+    finally:
+        K.set_pdl(old)
+    assert all(torch.equal(o, out) for o in outs)
+
+
+@pytest.mark.parametrize("T,nq,nkv,D,ctx", [(64, 64, 1, 128, [900, 5]), (64, 64, 1, 64, [300]), (4, 8, 1, 128, [20011]),
+                                            (16, 16, 2, 64, [9000, 70])])
+def test_tree_attention_of_many_rows_and_long_contexts(cuda, T, nq, nkv, D, ctx):
+    """Up to sixteen row blocks of a KV head, and contexts far beyond one tile per share; the same bits every time."""
+    g = gen(cuda, T + D)
+    q, kc, vc, bt, cl, bits = make_tree(g, cuda, len(ctx), T, nq, nkv, D, ctx, torch.float16)
+    y = K.tree_attention(q, kc, vc, bt, cl, bits, D ** -0.5)
+    ref, mag, sm = tree_ref(q, kc, vc, bt, cl, bits.tolist(), D ** -0.5)
+    check_tree(y, ref, mag, sm, max(ctx) + T, D)
+    for _ in range(10):
+        assert torch.equal(K.tree_attention(q, kc, vc, bt, cl, bits, D ** -0.5), y)

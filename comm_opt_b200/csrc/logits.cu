@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
   }
   // bit words of the chunk's ids v0 + 32 w ..: allowed, and touched by the history or a bias
   constexpr int kWords = MAXV * N * kThreads / 32, kPer = (kWords + kThreads - 1) / kThreads;
-  __shared__ uint32_t s_mask[kWords], s_mark[kWords + 1];  // (one more for the ids before v0)
+  __shared__ uint32_t s_mask[kWords], s_mark[kWords];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int w = tid + i * kThreads;
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kThreads) k_penalize(const __grid_constant__ L
   const int words4 = ((counts ? slots : 0) + (biases ? slots : 0)) / 4;
   for (int i = tid; i < words4; i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
   const int gs = p.vocab_offset - base;  // global id of slot 0
-  auto mark = [&](int slot) {
+  auto mark = [&](int slot) {  // (the ids before v0 look their tables up without it)
     if (slot >= N) atomicOr(&s_mark[(slot - N) >> 5], 1u << ((slot - N) & 31));
   };
   // biases in tiles of one entry per thread; each warp takes the ids of one residue and adds them up 32 entries at a

@@ -672,7 +672,7 @@ int log2_of(int x) {
   while ((1 << r) < x) ++r;
   return r;
 }
-// rows < 2^31 / seq * ... : the high word is exact while rows * seq < 2^32
+// the high word of row * inverse is row / seq for all rows below `rows` while rows * seq < 2^32; else 0, and the kernels divide
 uint32_t inverse_of(long long rows, int seq) {
   return seq > 1 && rows * seq < (1ll << 32) ? (uint32_t)(((1ull << 32) + seq - 1) / seq) : 0u;
 }

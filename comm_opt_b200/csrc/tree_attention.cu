@@ -215,8 +215,8 @@ __device__ __forceinline__ void quad_transpose(uint4 (&v)[4], int lane) {
 }
 
 // Bounded wait of a whole warp, one verdict for all lanes (and reconverged: the TMEM accesses that follow need it). The
-// timer and the failure flag are only looked at every 64 tries. Every waiter of a barrier sees every phase of it in turn,
-// so the parity is never ambiguous.
+// timer and the failure flag are only looked at every 64 tries. Every waiter of a barrier sees every phase of it in turn, so
+// the parity is never ambiguous (but for the softmax's waits for V tiles, where it is for another reason, stated there).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* fail, uint64_t limit) {
   uint64_t t0 = 0;
   for (uint32_t tries = 1;; ++tries) {
@@ -573,6 +573,10 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
           constexpr int CELLS = C::HALVES * 8 * C::STEP / 128;
           const int vs = i % C::VS, at = threadIdx.x % C::STEP, sr = st % C::PER * C::STEP + at, slot = s0 + at;
           const int part = threadIdx.x / C::STEP;
+          // These warps skip the phases of tiles without a tail, but the one before this is over all the same: the scores just
+          // seen were issued after the P V of two steps ago (a piece's first two after all of the previous piece's), which had
+          // waited for a V tile that is later than the one that held this stage before.
+          static_assert(C::VS >= 2 && C::PER <= 2, "the parity of v_full");
           okay = warp_wait(&v_full[vs], (i / C::VS) & 1, s_fail, p.timeout_ns);
           if (!okay) break;
           if (slot >= sl.ctx) {

@@ -70,9 +70,10 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: tor
     """Rotate x [tokens, heads, D] or [batch, seq, heads, D] (fp32, fp16, bf16; any strides) by its positions
     (int32 [seq] or [batch, seq]) and the tables cos, sin (fp32 [max_pos, rotary_dim / 2], see `rotary_tables`).
 
-    Differentiable in x (reverse mode). ``inverse`` applies the transpose, the gradient's rotation: it rotates back
-    where cos^2 + sin^2 = 1, and with tables that carry a factor m (YaRN's attention_factor) leaves m^2 x. ``out`` may be x (in place, no gradient) or other memory. A row whose
-    position lies outside the tables becomes zeros (and has a zero gradient): padded rows carry position -1."""
+    Differentiable in x (reverse mode). ``inverse`` applies the transpose, the gradient's rotation: it rotates back where
+    cos^2 + sin^2 = 1, and with tables that carry a factor m (YaRN's attention_factor) leaves m^2 x. ``out`` may be x (in
+    place, no gradient) or other memory. A row whose position lies outside the tables becomes zeros (and has a zero
+    gradient): padded rows carry position -1."""
     if out is None and x.requires_grad and torch.is_grad_enabled():
         return native().rotary_autograd(x, positions, cos, sin, bool(interleaved), bool(inverse))
     if out is not None and torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
@@ -113,7 +114,8 @@ def qk_norm_rotary_append_kv(qkv, positions, cos, sin, block_tables, starts, q_o
     starts[b] + s (int32 [batch]) and is rotated by positions[b, s] (int32; a drafted token's position is its depth, not
     its slot). q_out [batch, seq, nq, D]; caches [num_blocks, nkv, 16, D] (fp32, fp16, bf16) paged by block_tables
     [batch, max_blocks]. Rows s >= lens[b], and rows whose position lies outside the tables, are left out: q_out and the
-    caches keep what they held. k and v of rows whose slot or page does not exist are dropped. No gradient is formed."""
+    caches keep what they held. k and v of rows whose slot or page does not exist are dropped; the rows of a call have
+    slots of their own. No gradient is formed."""
     native().qk_norm_rotary_append(qkv, positions, cos, sin, block_tables, starts, q_out, k_cache, v_cache, int(nq),
                                    int(nkv), q_weight, k_weight, float(eps), lens, bias, bool(interleaved))
     return q_out

@@ -37,11 +37,11 @@ def tree_attention(q, k_cache, v_cache, block_tables, ctx_lens, tree_mask, scale
     block_tables int32 [batch, max_blocks]; ctx_lens int32 [batch]: tokens before the tree. Row t of sequence b sees
     the slots [0, ctx_lens[b]) and the drafted tokens j (slot ctx_lens[b] + j) with bit j of tree_mask (int64 [batch,
     tree] or [tree], see `tree_mask`; None: a chain, token t sees 0..t). A row that sees nothing gives zeros; whatever a
-    slot that a row does not see holds, infinities and NaN included, does not reach it. With tree_lens (int32 [batch]) rows t >=
-    tree_lens[b] are padding: nothing sees them and `out` keeps what it held there (zeros without `out`). Slots past
-    the block table are not seen; a page index outside the cache reads as zeros. Every wait inside the kernel is bounded by
-    `timeout_ms` (0: it gives up before the first): where one runs out, rows become NaN and `tree_attention_error_word` is
-    set. No gradient is formed."""
+    slot that a row does not see holds, infinities and NaN included, does not reach it. With tree_lens (int32 [batch])
+    rows t >= tree_lens[b] are padding: nothing sees them and `out` keeps what it held there (zeros without `out`). Slots
+    past the block table are not seen; a page index outside the cache reads as zeros. Every wait inside the kernel is
+    bounded by `timeout_ms` (0: it gives up before the first): where one runs out, rows become NaN and
+    `tree_attention_error_word` is set. No gradient is formed."""
     return native().tree_attention(q, k_cache, v_cache, block_tables, ctx_lens, tree_mask, float(scale), tree_lens, out,
                                    int(timeout_ms * 1e6))
 

@@ -16,9 +16,12 @@
 // coefficients once per row; every output is rounded once, at its store.
 //
 // Measured on one B200: 32763 rows of 64 fp16 heads, half of each rotated (1.08 GB): 169 us, 6.4 TB/s, the rate of a copy.
-// With the norm the instructions weigh as much as the bytes: 8 x 2048 rows of 32 + 8 bf16 heads, forward and backward with
-// the weights' gradients (841 MB): 193 us, 4.4 TB/s; padded prompts of 4 x 2048 rows into the cache: 47 us. 8 rows of one
-// decode step: 2.1 us (rotation), 2.6 us (norm, rotation, append): a launch.
+// With the norm neither memory nor the issue slots are full (backward: 50 and 38 %; prompts into the cache: 30 and 42 %): 12 to
+// 16 warps an SM have too few bytes on their way. 8 x 2048 rows of 32 + 8 bf16 heads, forward and backward with the weights'
+// gradients (841 MB): 194 us, 4.3 TB/s; padded prompts of 4 x 2048 rows into the cache: 47 us. 8 rows of one decode step: 1.8 us
+// (rotation), 2.6 us (norm, rotation, append): a launch. Narrow vectors are far from the bytes' rate, since their lanes are
+// given slots by the vector's width alone and most of them repeat the last: half layout, bf16 heads of 96 with 24 rotated 1.1
+// TB/s (interleaved, whose vectors stay wide, 5.2), fp32 heads of 80 with 20 rotated 0.8, heads of 64 off a 4-byte boundary 0.2.
 #include <algorithm>
 #include <type_traits>
 

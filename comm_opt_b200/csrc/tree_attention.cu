@@ -10,7 +10,7 @@
 // the softmax. S is written by the tensor cores into one of a row tile's two TMEM buffers, P goes back over it in 16 bits
 // and is the A operand of P V straight from TMEM; O stays in TMEM. Q K^T of the next step runs while the softmax works
 // on this one, which is what two buffers of 64 columns per row tile are for (one of 128 left the softmax waiting 1 us a
-// tile for its scores). O is rescaled only where a row's maximum rose by more than 2^8 (bf16; fp16 2^4, see kRise), which
+// tile for its scores; two of 128 fit beside one row tile's O, but not beside two). O is rescaled only where a row's maximum rose by more than 2^8 (bf16; fp16 2^4, see kRise), which
 // after the first tiles hardly happens; O / l is the same number.
 //
 // Work is cut into equal shares of the flattened (sequence, KV head, tile) space by the sequences' actual lengths,
@@ -19,14 +19,17 @@
 // L2. A (sequence, head) cut between shares leaves unnormalised partials (at most two per CTA) that a second kernel,
 // launched early, joins in the shares' order.
 //
-// Bounds, measured on one B200 at 4 x 64 drafted tokens over 32k, 64 / 8 heads of 128 (0.55 GB, 275 GFLOP): 276 us, 1.00
-// PFLOP/s. Without the softmax the same walk takes 222 us, of which Q K^T 97 us: M = 128, N = 64 from shared memory reads
+// Bounds, measured on one B200 at 4 x 64 drafted tokens over 32k, 64 / 8 heads of 128 (0.55 GB, 275 GFLOP): 270 us, 1.0
+// PFLOP/s, over the same inputs again and again, 326 us (0.84) with inputs that change from call to call. Without the softmax
+// the same walk takes 222 us, of which Q K^T 97 us: M = 128, N = 64 from shared memory reads
 // 6 KB per 32 cycles of arithmetic and the memory gives 128 bytes a cycle, but 128 columns do not fit beside O twice.
 // Exponentials on the FMA pipe (a degree-5 polynomial for 2 to 4 of 8), 16 softmax warps of 16 rows each (16x256b TMEM
 // accesses) and 128-column steps were all measured and no faster (288 - 303, 306, 305 us against 290 then); the two row
 // tiles taking turns at the exponential unit took it from 290 to 276.
-// Small: 8 drafted tokens over 1k, 32 / 8 heads: 10.8 us, latencies (lengths, page indices and first pages 3.2, one tile
-// 1.5, output 1, the join 3). 8 x 16 over up to 2k, 64 / 8 heads (38 MB): 21.5 us.
+// Small: 8 drafted tokens over 1k, 32 / 8 heads: 10.9 us, latencies (lengths, page indices and first pages 3.2, one tile
+// 1.5, output 1, the join 3). 8 x 16 over up to 2k, 64 / 8 heads (38 MB): 22 us. One row tile over long caches: 16 drafts over
+// 4 x 32k, 64 / 8 heads of 128: 109 us, 4.9 TB/s of cache; 8 x 8k, 32 / 8 heads: 60 us, 4.5 TB/s, and of 64 56 us, 2.4 TB/s
+// (the steps take as long with half the bytes, one CTA an SM).
 //
 // What a row does not see must not reach it, even when it is not finite: scores are replaced, not added to; slots past
 // the last token are zeroed in the V tile; a non-finite component of a drafted token's v is zeroed there too, and

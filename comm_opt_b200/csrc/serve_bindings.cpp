@@ -33,8 +33,15 @@ void ok(cudaError_t e, const char* what) { COB_CHECK(e == cudaSuccess, what, ": 
 
 cudaStream_t cur() { return at::cuda::getCurrentCUDAStream(); }
 
+// what the kernels read through its pointer is the tensor's value: no pending negation, no memory given back (a sharded
+// parameter between its uses) or never there
+void has_memory(const Tensor& t, const char* n) {
+  COB_CHECK(t.layout() == torch::kStrided && !t.is_neg(), n, " must be a strided tensor (a negated view: resolve_neg() first)");
+  COB_CHECK(!t._is_zerotensor() && (t.numel() == 0 || t.unsafeGetTensorImpl()->unsafe_storage().nbytes() > 0), n, " has no memory");
+}
 void on_device(const Tensor& t, const char* n, const Tensor& ref) {
   COB_CHECK(t.is_cuda() && t.device() == ref.device(), n, " must be a CUDA tensor on the device of the first operand");
+  has_memory(t, n);
 }
 
 // contiguous tensor of one type on the reference's device
@@ -169,6 +176,7 @@ void rows_of(const Tensor& x, const Tensor& pos, cob::RotaryParams& p) {
 
 void operand_ok(const Tensor& x, const char* n) {
   COB_CHECK(x.is_cuda(), n, " must be a CUDA tensor");
+  has_memory(x, n);
   COB_CHECK(x.dim() == 3 || x.dim() == 4, n, " must be [tokens, heads, head_dim] or [batch, seq, heads, head_dim]");
   code_of(x, n);
   head_dim_ok(x.size(-1));
@@ -379,6 +387,7 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
                               Tensor starts, Tensor q_out, Tensor k_cache, Tensor v_cache, int64_t nq, int64_t nkv,
                               OptTensor wq, OptTensor wk, double eps, OptTensor lens, OptTensor bias, bool interleaved) {
   COB_CHECK(qkv.is_cuda() && (qkv.dim() == 2 || qkv.dim() == 3), "qkv must be a CUDA tensor [batch, seq, width] or [batch * seq, width]");
+  has_memory(qkv, "qkv");
   code_of(qkv, "qkv");
   constants("qk_norm_rotary_append_kv", {&qkv, &q_out, &k_cache, &v_cache, given(wq), given(wk), given(bias)});
   COB_CHECK(nq >= 1 && nkv >= 1, "nq and nkv must be positive");
@@ -401,12 +410,8 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
   dense(q_out, "q_out", qkv.scalar_type(), qkv);
   COB_CHECK(q_out.numel() == B * S * nq * D, "q_out must hold batch x seq x nq x head_dim elements");
   cache_ok(k_cache, v_cache, block_tables, qkv, nkv, D, B);
-  apart({&q_out, &k_cache, &v_cache},
-        {&qkv, &positions, &cos_t, &sin_t, &block_tables, &starts, given(wq), given(wk), given(lens), given(bias)},
-        "q_out and the caches must lie in memory of their own");
   COB_CHECK(wq.has_value() == wk.has_value(), "give both norm weights or neither");
   cob::RotaryParams p;
-  Tensor like = qkv;  // type and device of the operands; head_dim components
   if (wq.has_value()) {
     for (const auto* w : {&*wq, &*wk}) {
       on_device(*w, "norm weight", qkv);
@@ -428,6 +433,9 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
     COB_CHECK(bias->numel() == W, "bias must have (nq + 2 nkv) * head_dim elements");
     p.bias = bias->data_ptr();
   }
+  apart({&q_out, &k_cache, &v_cache},
+        {&qkv, &positions, &cos_t, &sin_t, &block_tables, &starts, given(wq), given(wk), given(lens), given(bias)},
+        "q_out and the caches must lie in memory of their own");
   if (B * S == 0) return;
   const c10::cuda::CUDAGuard g(qkv.device());
   const int64_t e = qkv.element_size();
@@ -473,6 +481,7 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
 Tensor py_tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor ctx_lens, OptTensor mask,
                          double scale, OptTensor tree_lens, OptTensor out, int64_t timeout_ns) {
   COB_CHECK(q.is_cuda() && q.dim() == 4, "q must be a CUDA tensor [batch, tree, nq, head_dim]");
+  has_memory(q, "q");
   const int dtype = code_of(q, "q");
   COB_CHECK(dtype != cob::kF32, "q and the caches must be float16 or bfloat16");
   constants("tree_attention", {&q, &k_cache, &v_cache, given(out)});
@@ -559,6 +568,7 @@ Tensor py_penalize_logits(Tensor logits, OptTensor tokens, OptTensor lens, OptTe
   // the kernel looks up to 2048 entries ahead in 32-bit indexes, which must not wrap
   constexpr int64_t kMostEntries = 1ll << 30;
   COB_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be a CUDA tensor [rows, vocab]");
+  has_memory(logits, "logits");
   cob::LogitsParams p;
   p.dtype = code_of(logits, "logits");
   constants("penalize_logits", {&logits, given(repetition), given(frequency), given(presence), given(bias), given(out)});

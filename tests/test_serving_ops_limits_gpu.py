@@ -613,3 +613,49 @@ def test_tree_attention_of_many_rows_and_long_contexts(cuda, T, nq, nkv, D, ctx)
     check_tree(y, ref, mag, sm, max(ctx) + T, D)
     for _ in range(10):
         assert torch.equal(K.tree_attention(q, kc, vc, bt, cl, bits, D ** -0.5), y)
+
+
+def test_tensors_that_are_not_their_memory_are_refused(cuda):
+    """Lazily negated views, tensors whose storage was given back or never was, sparse ones: every operand."""
+    cos, sin = K.rotary_tables(64, 64, device=cuda)
+    pos = torch.arange(2, dtype=torch.int32, device=cuda)
+    x, w = torch.randn(2, 3, 64, device=cuda), torch.ones(64, device=cuda)
+    h = torch.randn(1, 2, 4, 64, device=cuda).half()
+    kc, vc = (torch.randn(3, 2, 16, 64, device=cuda).half() for _ in range(2))
+    bt, cl = torch.arange(2, dtype=torch.int32, device=cuda).view(1, 2), torch.zeros(1, dtype=torch.int32, device=cuda)
+    qkv, wh, b = torch.randn(1, 2, 512, device=cuda).half(), w.half(), torch.randn(512, device=cuda).half()
+    L, one = torch.randn(2, 64, device=cuda), torch.ones(2, device=cuda)
+    tok, bits = torch.zeros(2, 4, dtype=torch.int32, device=cuda), torch.full((2, 2), -1, dtype=torch.int32, device=cuda)
+    ids, bias = torch.zeros(2, 1, dtype=torch.int32, device=cuda), torch.ones(2, 1, device=cuda)
+    keys, mask = torch.zeros(2, dtype=torch.int64, device=cuda), torch.ones(2, dtype=torch.int64, device=cuda)
+    calls = [
+        (K.rotary, dict(x=x, positions=pos, cos=cos, sin=sin)),
+        (K.rotary, dict(x=x, positions=pos, cos=cos, sin=sin, out=torch.empty_like(x))),
+        (K.qk_norm_rotary, dict(q=x, k=x[:, :1].clone(), q_weight=w, k_weight=w.clone(), positions=pos, cos=cos, sin=sin)),
+        (K.qk_norm_rotary_backward, dict(dq=x.clone(), dk=x[:, :1].clone(), q=x, k=x[:, :1].clone(), q_weight=w, k_weight=w.clone(),
+                                         positions=pos, cos=cos, sin=sin)),
+        (K.qk_norm_rotary_append_kv, dict(qkv=qkv, positions=pos, cos=cos, sin=sin, block_tables=bt, starts=cl, q_out=h.clone(),
+                                          k_cache=kc, v_cache=vc, nq=4, nkv=2, q_weight=wh, k_weight=wh.clone(), lens=cl + 2, bias=b)),
+        (K.tree_attention, dict(q=h, k_cache=kc, v_cache=vc, block_tables=bt, ctx_lens=cl, tree_mask=mask, scale=1.0,
+                                tree_lens=cl + 2, out=torch.empty_like(h))),
+        (K.penalize_logits, dict(logits=L, tokens=tok, lens=tok[:, 0].clone(), prompt_lens=tok[:, 0].clone(), repetition=one,
+                                 frequency=one.clone(), presence=one.clone(), bias_ids=ids, bias=bias, allowed=bits, keys=keys,
+                                 out=torch.empty_like(L))),
+    ]
+    n = 0
+    for fn, kw in calls:
+        fn(**kw)
+        for name, t in kw.items():
+            if not torch.is_tensor(t):
+                continue
+            gone = t.clone()
+            gone.untyped_storage().resize_(0)
+            odd = [gone]
+            if t.is_floating_point():
+                odd += [torch._neg_view(t.clone()), t.to_sparse(), torch._efficientzerotensor(t.shape, dtype=t.dtype, device=cuda)]
+            for o in odd:
+                with pytest.raises(RuntimeError, match="memory|strided"):
+                    fn(**{**kw, name: o})
+                n += 1
+    assert n > 100
+    torch.cuda.synchronize()

@@ -181,6 +181,7 @@ void operand_ok(const Tensor& x, const char* n) {
   code_of(x, n);
   head_dim_ok(x.size(-1));
   for (int64_t i = 0; i < x.dim(); ++i) COB_CHECK(x.size(i) < (1ll << 31), n, " has a dimension past 2^31");
+  COB_CHECK(x.size(-2) <= (1 << 24), n, " has more than 2^24 heads");  // (sums of heads stay in 32 bits)
 }
 
 Tensor py_rotary(Tensor x, Tensor positions, Tensor cos_t, Tensor sin_t, bool interleaved, bool inverse, OptTensor out) {
@@ -390,7 +391,7 @@ void py_qk_norm_rotary_append(Tensor qkv, Tensor positions, Tensor cos_t, Tensor
   has_memory(qkv, "qkv");
   code_of(qkv, "qkv");
   constants("qk_norm_rotary_append_kv", {&qkv, &q_out, &k_cache, &v_cache, given(wq), given(wk), given(bias)});
-  COB_CHECK(nq >= 1 && nkv >= 1, "nq and nkv must be positive");
+  COB_CHECK(nq >= 1 && nkv >= 1 && nq <= (1 << 24) && nkv <= (1 << 24), "nq and nkv must be positive, at most 2^24");
   on_device(starts, "starts", qkv);
   const int64_t B = starts.numel(), W = qkv.size(-1), n = nq + 2 * nkv;
   COB_CHECK(W % n == 0, "qkv's rows must hold nq + 2 nkv heads");
@@ -575,7 +576,7 @@ Tensor py_penalize_logits(Tensor logits, OptTensor tokens, OptTensor lens, OptTe
   const int64_t B = logits.size(0), V = logits.size(1);
   COB_CHECK(V >= 1 && V <= (1 << 26) && B < (1ll << 31), "logits must be [rows, vocab] with 1 to 2^26 ids");
   COB_CHECK(logits.stride(1) == 1 || V == 1, "a row's logits must be contiguous");
-  COB_CHECK(vocab_offset >= 0 && vocab_offset + V < (1ll << 31), "vocab_offset must keep every id below 2^31");
+  COB_CHECK(vocab_offset >= 0 && vocab_offset < (1ll << 31) && vocab_offset + V < (1ll << 31), "vocab_offset must keep every id below 2^31");
   auto per_row = [&](const OptTensor& t, const char* n) -> const float* {
     if (!t.has_value()) return nullptr;
     dense(*t, n, torch::kFloat, logits);

@@ -659,3 +659,34 @@ def test_tensors_that_are_not_their_memory_are_refused(cuda):
                 n += 1
     assert n > 100
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("offset", [2 ** 31 - 64, 2 ** 31, 2 ** 63 - 1, 2 ** 63 - 64, -1])
+def test_vocabulary_offsets_that_wrap_are_refused(cuda, offset):
+    """Sums with 64-bit offsets do not wrap past the check (the mask would be read in front of its start)."""
+    x, bits = torch.zeros(1, 64, device=cuda), torch.full((1, 4), -1, dtype=torch.int32, device=cuda)
+    with pytest.raises(RuntimeError, match="vocab_offset"):
+        K.penalize_logits(x, allowed=bits, vocab_offset=offset)
+
+
+@pytest.mark.parametrize("nq,nkv", [(2 ** 63 - 2, 2 ** 62 + 1), (2 ** 62, 2 ** 61), (2 ** 40, 1), (0, 1), (1, -1)])
+def test_append_refuses_head_counts_that_wrap(cuda, nq, nkv):
+    """(the first sums to zero in 64 bits, which would divide the process to its end)"""
+    cos, sin = K.rotary_tables(8, 64, device=cuda)
+    z = torch.zeros(1, dtype=torch.int32, device=cuda)
+    kc = torch.zeros(2, 1, 16, 64, device=cuda)
+    with pytest.raises(RuntimeError, match="nq and nkv"):
+        K.qk_norm_rotary_append_kv(torch.zeros(1, 1, 256, device=cuda), z, cos, sin, z[None], z.clone(), torch.zeros(1, 1, 2, 64, device=cuda),
+                                   kc, kc.clone(), nq, nkv)
+
+
+def test_rotary_refuses_heads_whose_sums_wrap(cuda):
+    cos, sin = K.rotary_tables(8, 2, device=cuda)
+    pos, w = torch.zeros(1, dtype=torch.int32, device=cuda), torch.ones(2, device=cuda)
+    x = torch.zeros(1, 1, 2, device=cuda)
+    many = x.expand(1, 2 ** 31 - 1, 2)
+    with pytest.raises(RuntimeError, match="heads"):
+        K.rotary(many, pos, cos, sin)
+    for q, k in ((many, x), (x, many)):
+        with pytest.raises(RuntimeError, match="heads"):
+            K.qk_norm_rotary(q, k, w, w, pos, cos, sin)

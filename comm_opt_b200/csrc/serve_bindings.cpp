@@ -36,8 +36,11 @@ cudaStream_t cur() { return at::cuda::getCurrentCUDAStream(); }
 // what the kernels read through its pointer is the tensor's value: no pending negation, no memory given back (a sharded
 // parameter between its uses) or never there
 void has_memory(const Tensor& t, const char* n) {
-  COB_CHECK(t.layout() == torch::kStrided && !t.is_neg(), n, " must be a strided tensor (a negated view: resolve_neg() first)");
-  COB_CHECK(!t._is_zerotensor() && (t.numel() == 0 || t.unsafeGetTensorImpl()->unsafe_storage().nbytes() > 0), n, " has no memory");
+  constexpr c10::DispatchKeySet kOther({c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
+  const c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+  COB_CHECK(t.layout() == torch::kStrided && !(impl->key_set() & kOther).has_any(kOther) &&
+                (t.numel() == 0 || impl->unsafe_storage().nbytes() > 0),
+            n, " must be a strided tensor with memory of its values (a negated view: resolve_neg() first)");
 }
 void on_device(const Tensor& t, const char* n, const Tensor& ref) {
   COB_CHECK(t.is_cuda() && t.device() == ref.device(), n, " must be a CUDA tensor on the device of the first operand");

@@ -260,7 +260,7 @@ struct alignas(64) TreeArgs {
   int rb;              // row blocks of a (sequence, KV head)
   int shares;          // equal shares of the flattened (sequence, KV head, piece cost + tile) space
   float* part_o;       // [shares * rb][2][D / 4][ROWS][4]
-  float* part_ml;      // [shares * rb][2][ROWS][2]: maximum (times c) and sum
+  float* part_ml;      // [shares * rb][2][ROWS][2]: reference maximum and sum
 };
 
 struct SeqLen {
@@ -274,6 +274,9 @@ __device__ __forceinline__ SeqLen seq_len(const TreeAttnParams& p, int ctx, int 
   s.len = min(s.ctx + s.tl, cap);
   return s;
 }
+// scores to exponents of 2: a negative scale negates Q K^T in the MMA; a zero scale is a tiny one (masked scores are -inf: not
+// times 0)
+__device__ __forceinline__ float scale_log2(const TreeAttnParams& p) { return fmaxf(fabsf(p.scale) * kLog2e, 1e-37f); }
 __device__ __forceinline__ int token_of(int row, uint32_t inv) { return inv ? (int)__umulhi((uint32_t)row, inv) : row; }
 __device__ __forceinline__ int tiles_of(const SeqLen& s) { return s.tl > 0 ? (s.len + kTile - 1) / kTile : 0; }
 
@@ -512,8 +515,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
     const int row0 = rblk * C::ROWS + tile * 128 + wq * 32;  // first row of this warp
     const int r = row0 + lane;
     const int t_row = token_of(r, args.group_inv), g_row = r - t_row * args.group;
-    // a negative scale negates Q K^T in the MMA; a zero scale is a tiny one (masked scores are -inf: not times 0)
-    const float c = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
+    const float c = scale_log2(p);
     uint8_t* myQ = sQ + tile * C::TILE_BYTES;
     // this warp's 32 rows, 128-byte-swizzled K-major, missing rows as zeros: asynchronous, q_staged() ends it
     auto stage_q = [&](const Segment& s) {
@@ -659,13 +661,17 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
           }
           okay = my_turn(n);
           if (!okay) break;
-          const float mu = m == -INFINITY ? 0.f : m * c - kShift<T>;
-          const uint64_t c2 = pair(c, c), mu2 = pair(-mu, -mu);
+          // x = (s - m) c + kShift, the difference first: s c - m c would round m c, for large scores (2^24 and more) by more than
+          // the exponents that are left above P, and give infinities. The subtraction costs 2 % of the wide case; differences for
+          // the rows that need them alone, behind a branch, cost 7.
+          const float ref = m == -INFINITY ? 0.f : m;
+          const uint64_t ref2 = pair(-ref, -ref), c2 = pair(c, c), up2 = pair(kShift<T>, kShift<T>);
           uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
           for (int x = 0; x < 16 * G; ++x) {
             float a, b;
-            unpair(fma2(pair(__uint_as_float(s[x / 16][x % 16 * 2]), __uint_as_float(s[x / 16][x % 16 * 2 + 1])), c2, mu2), a, b);
+            const uint64_t d = add2(pair(__uint_as_float(s[x / 16][x % 16 * 2]), __uint_as_float(s[x / 16][x % 16 * 2 + 1])), ref2);
+            unpair(kShift<T> == 0.f ? mul2(d, c2) : fma2(d, c2, up2), a, b);
             a = ex2(a);
             b = ex2(b);
             sum[x & 1] = add2(sum[x & 1], pair(a, b));
@@ -755,7 +761,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
           }
         }
         if (live && !whole)
-          reinterpret_cast<float2*>(args.part_ml)[slot * C::ROWS + prow] = make_float2(m == -INFINITY ? -INFINITY : m * c, l);
+          reinterpret_cast<float2*>(args.part_ml)[slot * C::ROWS + prow] = make_float2(m, l);
       }
       tc_fence_before();
     }
@@ -786,7 +792,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::THREADS, 1) k_tree_attn(const __gr
 }
 
 // Joins the partials of (sequence, head) rows that were cut between shares, in the shares' order:
-// M = max m_i, out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i. A lane holds one row and 16 of its components, so
+// M = max m_i, out = sum 2^((m_i - M) c) O_i / sum 2^((m_i - M) c) l_i. A lane holds one row and 16 of its components, so
 // that the partials' vectors are read 512 bytes at a time and a row is written by whole sectors.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(128) k_tree_join(const __grid_constant__ TreeArgs args) {
@@ -814,6 +820,7 @@ __global__ void __launch_bounds__(128) k_tree_join(const __grid_constant__ TreeA
   auto slot = [&](int s) { return (size_t)(s * args.rb + rblk) * 2 + (s == s0 ? first : 0); };
   const float2* ml = reinterpret_cast<const float2*>(args.part_ml) + rr;
   const float4* po = reinterpret_cast<const float4*>(args.part_o) + (size_t)part * 4 * C::ROWS + rr;
+  const float c = scale_log2(p);
   float M = -INFINITY, L = 0.f;
   float4 o[4];
 #pragma unroll
@@ -835,7 +842,7 @@ __global__ void __launch_bounds__(128) k_tree_join(const __grid_constant__ TreeA
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) mn = fmaxf(mn, e[q].x);
     if (mn > M) {
-      const float f = exp2f(M - mn);
+      const float f = exp2f((M - mn) * c);
       M = mn;
       L *= f;
 #pragma unroll
@@ -844,7 +851,7 @@ __global__ void __launch_bounds__(128) k_tree_join(const __grid_constant__ TreeA
 #pragma unroll
     for (int q = 0; q < kBatch; ++q)
       if (e[q].x != -INFINITY) {  // (a piece in which the row sees nothing, or no piece)
-        const float f = exp2f(e[q].x - M);
+        const float f = exp2f((e[q].x - M) * c);
         L += f * e[q].y;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {

@@ -690,3 +690,32 @@ def test_rotary_refuses_heads_whose_sums_wrap(cuda):
     for q, k in ((many, x), (x, many)):
         with pytest.raises(RuntimeError, match="heads"):
             K.qk_norm_rotary(q, k, w, w, pos, cos, sin)
+
+
+# ----------------------------------------------------------------------------------------------- huge scores
+@pytest.mark.parametrize("dtype,mag", [(torch.float16, 2.0 ** 12), (torch.float16, 2.0 ** 15), (torch.bfloat16, 2.0 ** 13),
+                                       (torch.bfloat16, 2.0 ** 40), (torch.bfloat16, 2.0 ** 63)])
+@pytest.mark.parametrize("D,T,G,ctx", [(64, 3, 2, [200]), (128, 40, 8, [3000, 130])])
+def test_tree_attention_of_huge_scores(cuda, dtype, mag, D, T, G, ctx):
+    """Scores up to 2^127, far past where fp32 resolves a unit: every row is the mean of the values of its largest keys.
+
+    q has one component `mag`, keys one component 0.75, 1 or (two tokens a sequence) 1.5 times mag: scores of three values
+    exact in fp32, at least mag^2 / 8 apart, so every weight but those of the largest is zero or one, exactly."""
+    g = gen(cuda, D)
+    q, kc, vc, bt, cl, bits = make_tree(g, cuda, len(ctx), T, G, 1, D, ctx, dtype)
+    B = len(ctx)
+    q.zero_()
+    q[..., 7] = mag
+    kc.zero_()
+    n = max(ctx)
+    level = 0.75 + 0.25 * (torch.rand(B, n, generator=g, device=cuda) < 0.5)
+    want = torch.empty(B, D, dtype=torch.float64, device=cuda)
+    for b in range(B):
+        level[b, [3, ctx[b] - 2]] = 1.5
+        at = torch.arange(ctx[b], device=cuda)
+        kc[bt[b, at // 16].long(), 0, at % 16, 7] = (mag * level[b, :ctx[b]]).to(dtype)
+        want[b] = (vc[bt[b, 0].long(), 0, 3].double() + vc[bt[b, (ctx[b] - 2) // 16].long(), 0, (ctx[b] - 2) % 16].double()) / 2
+    for scale in (1.0, 0.125):
+        y = K.tree_attention(q, kc, vc, bt, cl, bits, scale)
+        ref = want[:, None, None].expand(y.shape)
+        close(y, ref, 4 * F32U * (ref.abs() + float(vc.abs().max())))

@@ -19,16 +19,16 @@
 // L2. A (sequence, head) cut between shares leaves unnormalised partials (at most two per CTA) that a second kernel,
 // launched early, joins in the shares' order.
 //
-// Bounds, measured on one B200 at 4 x 64 drafted tokens over 32k, 64 / 8 heads of 128 (0.55 GB, 275 GFLOP): 270 us, 1.0
-// PFLOP/s, over the same inputs again and again, 326 us (0.84) with inputs that change from call to call. Without the softmax
+// Bounds, measured on one B200 at 4 x 64 drafted tokens over 32k, 64 / 8 heads of 128 (0.55 GB, 275 GFLOP): 280 us, 0.98
+// PFLOP/s, over the same inputs again and again, 335 us (0.82) with inputs that change from call to call. Without the softmax
 // the same walk takes 222 us, of which Q K^T 97 us: M = 128, N = 64 from shared memory reads
 // 6 KB per 32 cycles of arithmetic and the memory gives 128 bytes a cycle, but 128 columns do not fit beside O twice.
 // Exponentials on the FMA pipe (a degree-5 polynomial for 2 to 4 of 8), 16 softmax warps of 16 rows each (16x256b TMEM
 // accesses) and 128-column steps were all measured and no faster (288 - 303, 306, 305 us against 290 then); the two row
 // tiles taking turns at the exponential unit took it from 290 to 276.
-// Small: 8 drafted tokens over 1k, 32 / 8 heads: 10.9 us, latencies (lengths, page indices and first pages 3.2, one tile
+// Small: 8 drafted tokens over 1k, 32 / 8 heads: 11.0 us, latencies (lengths, page indices and first pages 3.2, one tile
 // 1.5, output 1, the join 3). 8 x 16 over up to 2k, 64 / 8 heads (38 MB): 22 us. One row tile over long caches: 16 drafts over
-// 4 x 32k, 64 / 8 heads of 128: 109 us, 4.9 TB/s of cache; 8 x 8k, 32 / 8 heads: 60 us, 4.5 TB/s, and of 64 56 us, 2.4 TB/s
+// 4 x 32k, 64 / 8 heads of 128: 112 us, 4.8 TB/s of cache; 8 x 8k, 32 / 8 heads: 60 us, 4.5 TB/s, and of 64 56 us, 2.4 TB/s
 // (the steps take as long with half the bytes, one CTA an SM).
 //
 // What a row does not see must not reach it, even when it is not finite: scores are replaced, not added to; slots past
